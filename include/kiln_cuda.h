@@ -86,6 +86,13 @@ KC_API int kc_sync(kc_ctx_t ctx);
  * CUDA events or enqueue their own copies. */
 KC_API void* kc_ctx_stream(kc_ctx_t ctx);
 
+/* Order between the context's stream and another one (a cudaStream_t of the same device; NULL: the legacy default stream),
+ * without the host waiting: what the context is given after kc_ctx_wait_stream runs behind what `stream` holds now; what
+ * `stream` is given after kc_stream_wait_ctx runs behind what the context's stream holds now. Around an entry point that does
+ * not synchronise the two make it part of `stream`, also of one that is being captured into a graph. */
+KC_API int kc_ctx_wait_stream(kc_ctx_t ctx, void* stream);
+KC_API int kc_stream_wait_ctx(kc_ctx_t ctx, void* stream);
+
 /* Device status word: 0 when no kernel has recorded a bounded-wait failure
  * since the last call; otherwise a code naming the kernel and the wait that
  * gave up. Reading clears it. */
@@ -247,6 +254,31 @@ KC_API int kc_forward_step(kc_model_t model, kc_kv_t kv, const uint32_t* token_i
 KC_API int kc_greedy_rows(kc_ctx_t ctx, const void* logits_dev, int32_t rows, int32_t vocab,
                           int32_t normalize, uint32_t* tokens_out_dev);
 
+/* How a row's token is drawn. Tokens of a row stand in order of their logit, the largest first, the lower index first among
+ * equals (-0 is +0); w = exp((logit - largest) / temperature). top_k keeps the first top_k tokens (0: all), top_p the fewest of
+ * those whose weights reach top_p of theirs (1: all), min_p of these the ones of w >= min_p (0: all), one token at the least.
+ * Drawn is the first token whose running sum of weights exceeds u times the sum over what is kept, u in [0, 1) being the
+ * row's random number. temperature 0: the largest logit's token, the lowest index among equals. Masked tokens (-inf) and NaN
+ * are never drawn, beside +inf nothing else is; a row that has nothing but those gives token 0 and log probability -inf. */
+typedef struct {
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} kc_sampling;
+
+/* A token drawn per logits row, beside kc_greedy_rows (Sampler's categorical lane, crates/kiln-engine/src/sampler.rs, with the
+ * random numbers given instead of a key). logits_dev: bf16, `ld` values from row to row (any alignment of 2 bytes);
+ * sampling_dev: device kc_sampling [rows], 16-byte aligned; uniform_dev: device f32 [rows]; tokens_out_dev: device u32 [rows];
+ * logprobs_out_dev: device f32 [rows], or NULL: the logarithm of the drawn token's share of the kept tokens' weights (0 at
+ * temperature 0). Settings are on the device and not refused: a temperature that is not positive is 0, a top_k below 1 all
+ * tokens, a top_p of 1 and more or NaN all, of 0 and less the first token, a min_p that is not positive all; u below 0 is the first token,
+ * of 1 and more or NaN the last one kept. Weights and sums are in 64 bits, and a row's result depends on nothing but the row and its
+ * settings. Asynchronous on the context's stream; no workspace, so that it may be captured and several may run at once. */
+KC_API int kc_sample_rows(kc_ctx_t ctx, const void* logits_dev, int64_t ld, int32_t rows, int32_t vocab,
+                          const kc_sampling* sampling_dev, const float* uniform_dev, uint32_t* tokens_out_dev,
+                          float* logprobs_out_dev);
+
 /* Device form of the settle walk (engine.rs:2336-2383) for n_seqs verify
  * segments. Row tokens of segment i start at seq_row_offsets[i] and number
  * draft_len[i]+1; draft tokens start at draft_offsets[i]. Outputs per segment:
@@ -273,6 +305,18 @@ KC_API int kc_verify_step(kc_model_t model, kc_kv_t kv, const uint32_t* token_id
                           const kc_seq_step* seqs, int32_t n_seqs,
                           uint32_t* row_tokens_out, int32_t* n_committed_out,
                           int32_t* n_accepted_out);
+
+/* kc_verify_step for sequences that sample: row j of sequence i is drawn by sampling[i] with its own random number (HOST
+ * arrays: sampling [n_seqs]; uniform [n_sampled], in the order of the sampled rows), or, at temperature 0, is the greedy row of
+ * kc_verify_step. The walk is the same. A drafter proposes a token, not a distribution, so a drawn row that has to equal the
+ * draft is speculative sampling's acceptance: a draft d is accepted with probability p(d), and what a row commits instead
+ * of it is distributed as p without d. Rows of a sequence that does not speculate are drawn from the same distribution.
+ * Refused: a temperature, top_p or min_p that is negative, NaN or infinite, a top_p of 0 or past 1, a min_p past 1, a negative
+ * top_k, a random number outside [0, 1). logprobs_out: host f32 [n_sampled] or NULL, as in kc_sample_rows. */
+KC_API int kc_verify_step_sampled(kc_model_t model, kc_kv_t kv, const uint32_t* token_ids, int32_t n,
+                                  const kc_seq_step* seqs, int32_t n_seqs, const kc_sampling* sampling,
+                                  const float* uniform, uint32_t* row_tokens_out, float* logprobs_out,
+                                  int32_t* n_committed_out, int32_t* n_accepted_out);
 
 /* Pipelined plain decode (crates/kiln-engine/src/engine.rs:1428-1455 pipelined_turn, 1656-1744 build_pipelined,
  * 1748-1766 apply_inflight). kc_decode_launch queues ONE decode forward — every segment feeds one row and samples it,

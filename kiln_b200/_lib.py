@@ -44,6 +44,10 @@ class KcSeqStep(C.Structure):
                 ("blocks", C.POINTER(C.c_uint32))]
 
 
+class KcSampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
 _P = C.c_void_p
 _SIGNATURES = {
     "kc_ctx_create": (C.c_int, [C.c_int, C.POINTER(_P)]),
@@ -52,6 +56,8 @@ _SIGNATURES = {
     "kc_live_objects": (C.c_int64, []),
     "kc_sync": (C.c_int, [_P]),
     "kc_ctx_stream": (_P, [_P]),
+    "kc_ctx_wait_stream": (C.c_int, [_P, _P]),
+    "kc_stream_wait_ctx": (C.c_int, [_P, _P]),
     "kc_device_status": (C.c_int, [_P, C.POINTER(C.c_uint32)]),
     "kc_launch_count": (C.c_int64, [_P]),
     "kc_last_step_ms": (C.c_double, [_P]),
@@ -72,9 +78,13 @@ _SIGNATURES = {
     "kc_forward_step": (C.c_int, [_P, _P, C.POINTER(C.c_uint32), C.c_int32, C.POINTER(KcSeqStep), C.c_int32, C.c_int32,
                                   C.POINTER(_P), C.POINTER(C.c_int32)]),
     "kc_greedy_rows": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, _P]),
+    "kc_sample_rows": (C.c_int, [_P, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P]),
     "kc_verify_accept": (C.c_int, [_P, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, _P, _P, _P]),
     "kc_verify_step": (C.c_int, [_P, _P, C.POINTER(C.c_uint32), C.c_int32, C.POINTER(KcSeqStep), C.c_int32,
                                  C.POINTER(C.c_uint32), C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
+    "kc_verify_step_sampled": (C.c_int, [_P, _P, C.POINTER(C.c_uint32), C.c_int32, C.POINTER(KcSeqStep), C.c_int32, C.POINTER(KcSampling),
+                                         C.POINTER(C.c_float), C.POINTER(C.c_uint32), C.POINTER(C.c_float), C.POINTER(C.c_int32),
+                                         C.POINTER(C.c_int32)]),
     "kc_decode_launch": (C.c_int, [_P, _P, C.POINTER(C.c_uint32), C.POINTER(C.c_int32), C.POINTER(KcSeqStep), C.c_int32,
                                    C.POINTER(C.c_uint64)]),
     "kc_decode_collect": (C.c_int, [_P, C.c_uint64, C.POINTER(C.c_uint32), C.c_int32]),

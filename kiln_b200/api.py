@@ -217,6 +217,7 @@ class Context:
         # drops the Python objects in (a library handle must not outlive its context)
         self._children = weakref.WeakSet()
         check(L.lib().kc_ctx_create(device, C.byref(self._h)))
+        self._stream = self.stream
 
     def _adopt(self, child) -> None:
         self._children.add(child)
@@ -240,6 +241,21 @@ class Context:
     @property
     def stream(self) -> int:
         return int(L.lib().kc_ctx_stream(self._h) or 0)
+
+    def on_current_stream(self, call, *args) -> None:
+        """``call(handle, *args)``, an entry point that does not synchronise, as part of torch's current stream of this
+        context's device: behind what that stream and the context's hold, and ahead of what either is given later. The host
+        waits for nothing, also in a capture into a graph. A program that makes the context's stream torch's current one
+        (``torch.cuda.ExternalStream(ctx.stream)``) spares the two events that this takes."""
+        current = torch.cuda.current_stream(self.device).cuda_stream
+        if current == self._stream:
+            check(call(self._h, *args))
+            return
+        check(L.lib().kc_ctx_wait_stream(self._h, current))
+        try:
+            check(call(self._h, *args))
+        finally:
+            check(L.lib().kc_stream_wait_ctx(self._h, current))
 
     def device_status(self) -> int:
         st = C.c_uint32(0)
@@ -412,6 +428,23 @@ class CudaModel:
                                      nacc.ctypes.data_as(C.POINTER(C.c_int32))))
         return rows[:n_sampled], ncom, nacc
 
+    def verify_step_sampled(self, batch: StepBatch, kv: PagedKv, sampling: Sequence["SamplingParams"], uniforms: Sequence[float]):
+        """verify_step with drawn rows (kc_verify_step_sampled): a setting per sequence, a random number in [0, 1) per sampled
+        row. Returns (row_tokens[n_sampled], n_committed[n_seqs], n_accepted[n_seqs], logprobs[n_sampled])."""
+        p = _PackedStep(batch)
+        n_sampled = sum(s.sample_rows for s in batch.seqs)
+        u = np.ascontiguousarray(uniforms, dtype=np.float32)
+        if len(sampling) != p.n_seqs or u.shape != (n_sampled,):
+            raise ValueError(f"{p.n_seqs} sequences and {n_sampled} sampled rows have {len(sampling)} settings and random numbers {u.shape}")
+        settings = (L.KcSampling * max(1, p.n_seqs))(*[L.KcSampling(s.temperature, s.top_k, s.top_p, s.min_p) for s in sampling])
+        rows, logprobs = np.zeros(max(1, n_sampled), dtype=np.uint32), np.zeros(max(1, n_sampled), dtype=np.float32)
+        ncom, nacc = np.zeros(p.n_seqs, dtype=np.int32), np.zeros(p.n_seqs, dtype=np.int32)
+        as_f32, as_i32 = C.POINTER(C.c_float), C.POINTER(C.c_int32)
+        check(L.lib().kc_verify_step_sampled(self._h, kv._h, p.ids_p, p.n, p.seq_arr, p.n_seqs, settings, u.ctypes.data_as(as_f32),
+                                             rows.ctypes.data_as(C.POINTER(C.c_uint32)), logprobs.ctypes.data_as(as_f32),
+                                             ncom.ctypes.data_as(as_i32), nacc.ctypes.data_as(as_i32)))
+        return rows[:n_sampled], ncom, nacc, logprobs[:n_sampled]
+
     def decode_launch(self, batch: StepBatch, kv: PagedKv, feed: Sequence[int]) -> int:
         """Queues one pipelined decode step (engine.rs:1656-1744) and returns its ticket; feed[i] >= 0 takes sequence
         i's input id from that row of the previous launch, still on the device."""
@@ -495,6 +528,60 @@ def greedy_rows(ctx: Context, logits: torch.Tensor, normalize: bool = True) -> t
     check(L.lib().kc_greedy_rows(ctx._h, logits.data_ptr(), logits.shape[0], logits.shape[1], int(normalize), out.data_ptr()))
     ctx.sync()
     return out
+
+
+@dataclass(frozen=True)
+class SamplingParams:
+    """How a request's tokens are drawn (kc_sampling); temperature 0 is greedy, and the defaults keep every token."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+    def __post_init__(self):
+        if not (0.0 <= self.temperature < float("inf")):
+            raise ValueError(f"temperature {self.temperature}: 0 or a positive number")
+        if not (0 <= self.top_k < 1 << 31):
+            raise ValueError(f"top_k {self.top_k}: 0 (all) or a number of tokens")
+        if not (0.0 < self.top_p <= 1.0):
+            raise ValueError(f"top_p {self.top_p}: in (0, 1]")
+        if not (0.0 <= self.min_p <= 1.0):
+            raise ValueError(f"min_p {self.min_p}: in [0, 1]")
+
+
+_SAMPLING = np.dtype([("temperature", "f4"), ("top_k", "i4"), ("top_p", "f4"), ("min_p", "f4")])
+
+
+def pack_sampling(params: Sequence[SamplingParams], device) -> torch.Tensor:
+    """The settings of a batch's rows as sample_rows takes them, int32 [rows, 4] on the device: made once, kept while they hold."""
+    rec = np.array([(p.temperature, p.top_k, p.top_p, p.min_p) for p in params], dtype=_SAMPLING)
+    return torch.from_numpy(rec.view(np.int32).reshape(-1, 4)).to(device)
+
+
+def sample_rows(ctx: Context, logits: torch.Tensor, params, uniforms: torch.Tensor, out: Optional[torch.Tensor] = None,
+                logprobs: Optional[torch.Tensor] = None):
+    """A token drawn per row of logits (bf16 [rows, vocab], rows at any stride) and its log probability among the tokens that
+    were kept: (int32 [rows], float32 [rows]); see kc_sample_rows. ``params``: pack_sampling's tensor or a sequence of
+    SamplingParams; ``uniforms``: float32 [rows] in [0, 1) on the device. ``out`` and ``logprobs``: where the results go.
+    Part of torch's current stream (Context.on_current_stream); the host does not wait."""
+    if logits.dtype != torch.bfloat16 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits: bf16 [rows, vocab], the values of a row side by side")
+    rows, vocab = logits.shape
+    if not isinstance(params, torch.Tensor):
+        params = pack_sampling(params, logits.device)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    if logprobs is None:
+        logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    for name, t, dtype, shape in (("params", params, torch.int32, (rows, 4)), ("uniforms", uniforms, torch.float32, (rows,)),
+                                  ("out", out, torch.int32, (rows,)), ("logprobs", logprobs, torch.float32, (rows,))):
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous {dtype} {list(shape)}")
+    if any(t.device.type != "cuda" or t.device.index != ctx.device for t in (logits, params, uniforms, out, logprobs)):
+        raise ValueError(f"tensors of a context on cuda:{ctx.device}")
+    ctx.on_current_stream(L.lib().kc_sample_rows, logits.data_ptr(), logits.stride(0), rows, vocab, params.data_ptr(), uniforms.data_ptr(),
+                          out.data_ptr(), logprobs.data_ptr())
+    return out, logprobs
 
 
 def verify_accept(ctx: Context, row_tokens: torch.Tensor, row_offsets: torch.Tensor, draft: torch.Tensor,

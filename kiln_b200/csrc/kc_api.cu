@@ -93,6 +93,7 @@ struct kc_ctx {
   // draft lane accounting (kc_draft_chain): host wall time of the calls and tokens proposed
   double draft_ms = 0.0;
   int64_t draft_tokens = 0, draft_calls = 0;
+  cudaEvent_t join = nullptr;               // kc_ctx_wait_stream, kc_stream_wait_ctx
   cudaEvent_t take_event() {
     if (!event_pool.empty()) { cudaEvent_t e = event_pool.back(); event_pool.pop_back(); return e; }
     cudaEvent_t e = nullptr;
@@ -160,7 +161,7 @@ struct Layer {
 
 // Per-step metadata, packed on the host and copied to the device in one transfer.
 struct MetaLayout {
-  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, total;
+  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, sampling, uniform, total;
 };
 
 struct kc_model {
@@ -273,6 +274,7 @@ extern "C" int kc_ctx_create(int device, kc_ctx_t* out) {
   *c->status_host = 0;
   cudaEventCreate(&c->step_a);
   cudaEventCreate(&c->step_b);
+  cudaEventCreateWithFlags(&c->join, cudaEventDisableTiming);
   g_live++;
   {
     std::lock_guard<std::mutex> lk(g_ctx_mu);
@@ -296,6 +298,7 @@ extern "C" void kc_ctx_destroy(kc_ctx_t c) {
   for (auto e : c->event_pool) cudaEventDestroy(e);
   cudaEventDestroy(c->step_a);
   cudaEventDestroy(c->step_b);
+  cudaEventDestroy(c->join);
   if (c->comm) ncclCommDestroy(c->comm);
   cudaFree(c->gemm_fix);
   free_op_shell(c);
@@ -339,6 +342,39 @@ extern "C" int kc_sync(kc_ctx_t c) {
 }
 
 extern "C" void* kc_ctx_stream(kc_ctx_t c) { return c ? (void*)c->stream : nullptr; }
+
+// The caller's device again at the end of a call: for entry points that run among other libraries' calls.
+struct OnDevice {
+  int before = -1;
+  cudaError_t enter(int device) {
+    int d = 0;
+    cudaError_t e = cudaGetDevice(&d);
+    if (e != cudaSuccess || d == device) return e;
+    e = cudaSetDevice(device);
+    if (e == cudaSuccess) before = d;
+    return e;
+  }
+  ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+};
+
+extern "C" int kc_ctx_wait_stream(kc_ctx_t c, void* stream) {
+  if (!c) return fail(KC_ERR_INVALID, "kc_ctx_wait_stream: ctx is NULL");
+  if (stream == (void*)c->stream) return KC_OK;
+  OnDevice on;
+  CK(on.enter(c->device));
+  CK(cudaEventRecord(c->join, (cudaStream_t)stream));
+  CK(cudaStreamWaitEvent(c->stream, c->join, 0));
+  return KC_OK;
+}
+extern "C" int kc_stream_wait_ctx(kc_ctx_t c, void* stream) {
+  if (!c) return fail(KC_ERR_INVALID, "kc_stream_wait_ctx: ctx is NULL");
+  if (stream == (void*)c->stream) return KC_OK;
+  OnDevice on;
+  CK(on.enter(c->device));
+  CK(cudaEventRecord(c->join, c->stream));
+  CK(cudaStreamWaitEvent((cudaStream_t)stream, c->join, 0));
+  return KC_OK;
+}
 
 extern "C" int kc_device_status(kc_ctx_t c, uint32_t* status) {
   if (!c || !status) return fail(KC_ERR_INVALID, "kc_device_status: NULL argument");
@@ -1000,7 +1036,7 @@ extern "C" int kc_model_load(kc_ctx_t c, const kc_model_desc* desc, const kc_ten
     cudaError_t e = cudaSuccess;
     if (e == cudaSuccess) e = cudaMalloc(&m->row_tokens, R * 4);
     if (e == cudaSuccess) e = cudaMalloc(&m->committed, R * 4);
-    if (e == cudaSuccess) e = cudaMallocHost(&m->result_host, R * 4 + (size_t)m->max_seqs * 8 + 64);
+    if (e == cudaSuccess) e = cudaMallocHost(&m->result_host, R * 8 + (size_t)m->max_seqs * 8 + 64);
     for (int i = 0; i < kc_model::kStaging && e == cudaSuccess; ++i) e = cudaEventCreateWithFlags(&m->meta_ev[i], cudaEventDisableTiming);
     for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
       e = cudaMalloc(&m->pipe_tokens[i], (size_t)m->max_seqs * 4);
@@ -1050,6 +1086,7 @@ struct StepPlan {
   int max_len = 1;
   bool whole = false;              // attention units hold all chunks of their rows
   bool keys = false;               // attention by the kernel with a key per thread
+  bool draws = false;              // sampled rows have settings and random numbers (kc_verify_step_sampled)
   std::vector<AttnUnit> units;
   MetaLayout lay{};
 };
@@ -1120,7 +1157,7 @@ std::vector<int> old_keys(kc_kv* kv, const kc_seq_step* seqs, int n_seqs) {
 }
 
 int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, const kc_seq_step* seqs, int32_t n_seqs,
-                  int32_t pad_rows, StepPlan* plan, bool alone = false, bool capped = false) {
+                  int32_t pad_rows, StepPlan* plan, bool alone = false, bool capped = false, bool draws = false) {
   if (!m || !kv || !token_ids || !seqs) return fail(KC_ERR_INVALID, "forward_step: NULL argument");
   if (kv->ctx != m->ctx) return fail(KC_ERR_INVALID, "forward_step: model and pools belong to different contexts");
   if (kv->layers != m->d.num_layers || kv->kv_heads != m->Hkv || kv->head_dim != m->d.head_dim)
@@ -1134,7 +1171,7 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
   if (n > m->max_rows) return fail(KC_ERR_INVALID, "step of %d tokens exceeds max_step_tokens %d", n, m->d.max_step_tokens);
   if (n_seqs > m->max_seqs) return fail(KC_ERR_INVALID, "step of %d sequences exceeds max_step_seqs %d", n_seqs, m->max_seqs);
   StepPlan p;
-  p.n = n; p.n_seqs = n_seqs;
+  p.n = n; p.n_seqs = n_seqs; p.draws = draws;
   int max_ctx = 1;
   for (int i = 0; i < n_seqs; ++i) {
     const kc_seq_step& s = seqs[i];
@@ -1168,6 +1205,7 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
   L.v_row_off = put((size_t)n_seqs * 4); L.v_draft_off = put((size_t)n_seqs * 4); L.v_draft_len = put((size_t)n_seqs * 4);
   L.v_draft = put((size_t)n * 4);
   L.feed = put((size_t)n * 4);
+  if (p.draws) { L.sampling = put((size_t)p.n_sampled * sizeof(kc_sampling)); L.uniform = put((size_t)p.n_sampled * 4); }
   L.total = at;
   *plan = std::move(p);
   return KC_OK;
@@ -1177,7 +1215,8 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
 // `before_copy` (optional) is recorded on the stream after the host-side packing and before the copy is queued: the
 // device span of a step starts there, so host packing time is not counted as device time.
 int upload_meta(kc_model* m, kc_kv* kv, const uint32_t* token_ids, const kc_seq_step* seqs, const StepPlan& p,
-                cudaEvent_t before_copy = nullptr, const int32_t* feed = nullptr) {
+                cudaEvent_t before_copy = nullptr, const int32_t* feed = nullptr, const kc_sampling* sampling = nullptr,
+                const float* uniform = nullptr) {
   kc_ctx* c = m->ctx;
   const MetaLayout& L = p.lay;
   if (L.total > m->meta_cap) {
@@ -1206,6 +1245,11 @@ int upload_meta(kc_model* m, kc_kv* kv, const uint32_t* token_ids, const kc_seq_
   uint32_t* v_draft = reinterpret_cast<uint32_t*>(hbuf + L.v_draft);
   memcpy(tokens, token_ids, (size_t)p.n * 4);
   if (feed) memcpy(hbuf + L.feed, feed, (size_t)p.n * 4);
+  if (p.draws) {
+    memcpy(hbuf + L.uniform, uniform, (size_t)p.n_sampled * 4);
+    kc_sampling* of_row = reinterpret_cast<kc_sampling*>(hbuf + L.sampling);
+    for (int i = 0; i < p.n_seqs; ++i) of_row = std::fill_n(of_row, seqs[i].sample_rows, sampling[i]);
+  }
   const int BS = kv->block_size;
   int row = 0, srow = 0, dat = 0;
   for (int i = 0; i < p.n_seqs; ++i) {
@@ -1508,6 +1552,22 @@ extern "C" int kc_greedy_rows(kc_ctx_t c, const void* logits_dev, int32_t rows, 
   return KC_OK;
 }
 
+static_assert(sizeof(kc_sampling) == sizeof(DrawSetting) && alignof(DrawSetting) == 16, "a row's settings are read as one vector");
+
+extern "C" int kc_sample_rows(kc_ctx_t c, const void* logits_dev, int64_t ld, int32_t rows, int32_t vocab, const kc_sampling* sampling_dev,
+                              const float* uniform_dev, uint32_t* tokens_out_dev, float* logprobs_out_dev) {
+  if (!c || !logits_dev || !sampling_dev || !uniform_dev || !tokens_out_dev) return fail(KC_ERR_INVALID, "kc_sample_rows: NULL argument");
+  if (rows < 1 || vocab < 1 || vocab > 1 << 30) return fail(KC_ERR_INVALID, "kc_sample_rows: [%d, %d]", rows, vocab);
+  if (ld < vocab && rows > 1) return fail(KC_ERR_INVALID, "kc_sample_rows: rows of %d values every %lld", vocab, (long long)ld);
+  if ((uintptr_t)logits_dev % 2 || (uintptr_t)sampling_dev % 16 || (uintptr_t)uniform_dev % 4 || (uintptr_t)tokens_out_dev % 4 || (uintptr_t)logprobs_out_dev % 4)
+    return fail(KC_ERR_INVALID, "kc_sample_rows: an argument is not aligned (logits 2 bytes, settings 16, the others 4)");
+  OnDevice on;
+  CK(on.enter(c->device));
+  LAUNCH(c, KC_PROF_SAMPLE, 1, launch_draw_rows((const bf16*)logits_dev, ld, rows, vocab, reinterpret_cast<const DrawSetting*>(sampling_dev), uniform_dev,
+                                                tokens_out_dev, logprobs_out_dev, c->sm_count, c->stream));
+  return KC_OK;
+}
+
 extern "C" int kc_verify_accept(kc_ctx_t c, const uint32_t* row_tokens_dev, const int32_t* seq_row_offsets_dev,
                                 const uint32_t* draft_dev, const int32_t* draft_offsets_dev, const int32_t* draft_len_dev,
                                 int32_t n_seqs, int32_t max_commit, uint32_t* committed_out_dev,
@@ -1522,20 +1582,37 @@ extern "C" int kc_verify_accept(kc_ctx_t c, const uint32_t* row_tokens_dev, cons
   return KC_OK;
 }
 
-extern "C" int kc_verify_step(kc_model_t m, kc_kv_t kv, const uint32_t* token_ids, int32_t n, const kc_seq_step* seqs,
-                              int32_t n_seqs, uint32_t* row_tokens_out, int32_t* n_committed_out, int32_t* n_accepted_out) {
+// The verify round; with `sampling` rows are drawn (kc_verify_step_sampled).
+static int verify_round(const char* where, kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, const kc_seq_step* seqs, int32_t n_seqs,
+                        const kc_sampling* sampling, const float* uniform, uint32_t* row_tokens_out, float* logprobs_out,
+                        int32_t* n_committed_out, int32_t* n_accepted_out) {
   StepPlan p;
-  int rc = validate_step(m, kv, token_ids, n, seqs, n_seqs, 0, &p);
+  int rc = validate_step(m, kv, token_ids, n, seqs, n_seqs, 0, &p, false, false, sampling != nullptr);
   if (rc) return rc;
   kc_ctx* c = m->ctx;
+  bool greedy = sampling == nullptr, drawn = false;   // what the sampled rows need
+  if (sampling) {
+    for (int i = 0; i < n_seqs; ++i) {
+      const kc_sampling& s = sampling[i];
+      if (!(s.temperature >= 0.f && s.temperature < INFINITY) || s.top_k < 0 || !(s.top_p > 0.f && s.top_p <= 1.f) || !(s.min_p >= 0.f && s.min_p <= 1.f))
+        return fail(KC_ERR_INVALID, "%s: sequence %d samples with temperature %g, top_k %d, top_p %g, min_p %g", where, i, s.temperature, s.top_k, s.top_p, s.min_p);
+      if (seqs[i].sample_rows > 0) (s.temperature > 0.f ? drawn : greedy) = true;
+    }
+    for (int j = 0; j < p.n_sampled; ++j)
+      if (!(uniform[j] >= 0.f && uniform[j] < 1.f)) return fail(KC_ERR_INVALID, "%s: random number %g of row %d lies outside [0, 1)", where, uniform[j], j);
+  }
   CK(cudaSetDevice(c->device));
-  if ((rc = upload_meta(m, kv, token_ids, seqs, p, c->step_a))) return rc;
+  if ((rc = upload_meta(m, kv, token_ids, seqs, p, c->step_a, nullptr, sampling, uniform))) return rc;
   if ((rc = run_forward(m, kv, reinterpret_cast<const uint32_t*>(m->meta_dev + p.lay.tokens), p, true))) return rc;
   if (p.n_sampled > 0) {
     // The results go straight into the pinned result buffer (a few hundred bytes of posted writes): no copies follow.
     uint8_t* hb = m->result_host;
-    const size_t o1 = align_up((size_t)p.n_sampled * 4, 16), o2 = o1 + align_up((size_t)n_seqs * 4, 16);
-    LAUNCH(c, KC_PROF_SAMPLE, 1, launch_greedy_rows(m->logits, p.n_sampled, m->d.vocab_size, 1, m->row_tokens, c->stream, (uint32_t*)hb));
+    const size_t o1 = align_up((size_t)p.n_sampled * 4, 16), o2 = o1 + align_up((size_t)n_seqs * 4, 16), o3 = o2 + align_up((size_t)n_seqs * 4, 16);
+    if (greedy) LAUNCH(c, KC_PROF_SAMPLE, 1, launch_greedy_rows(m->logits, p.n_sampled, m->d.vocab_size, 1, m->row_tokens, c->stream, (uint32_t*)hb));
+    if (drawn)
+      LAUNCH(c, KC_PROF_SAMPLE, 1, launch_draw_rows(m->logits, m->d.vocab_size, p.n_sampled, m->d.vocab_size, reinterpret_cast<const DrawSetting*>(m->meta_dev + p.lay.sampling),
+                                                    reinterpret_cast<const float*>(m->meta_dev + p.lay.uniform), m->row_tokens, nullptr, c->sm_count, c->stream,
+                                                    (uint32_t*)hb, logprobs_out ? (float*)(hb + o3) : nullptr, 1));
     // max_commit = 0: the committed list is row_tokens[row_off .. row_off + n_committed), no second copy needed
     LAUNCH(c, KC_PROF_SAMPLE, 1, launch_verify_accept(m->row_tokens, reinterpret_cast<const int32_t*>(m->meta_dev + p.lay.v_row_off),
                             reinterpret_cast<const uint32_t*>(m->meta_dev + p.lay.v_draft),
@@ -1545,19 +1622,37 @@ extern "C" int kc_verify_step(kc_model_t m, kc_kv_t kv, const uint32_t* token_id
     CK(cudaEventRecord(c->step_b, c->stream));
     CK(cudaStreamSynchronize(c->stream));
     cudaEventElapsedTime(&c->last_step_ms, c->step_a, c->step_b);
-    RC(status_verdict(c, "kc_verify_step"));
+    RC(status_verdict(c, where));
     if (row_tokens_out) memcpy(row_tokens_out, hb, (size_t)p.n_sampled * 4);
     if (n_committed_out) memcpy(n_committed_out, hb + o1, (size_t)n_seqs * 4);
     if (n_accepted_out) memcpy(n_accepted_out, hb + o2, (size_t)n_seqs * 4);
+    if (logprobs_out && sampling) {
+      const float* from = (const float*)(hb + o3);
+      for (int i = 0, j = 0; i < n_seqs; ++i)
+        for (int k = 0; k < seqs[i].sample_rows; ++k, ++j) logprobs_out[j] = sampling[i].temperature > 0.f ? from[j] : 0.f;
+    }
   } else {
     CK(cudaEventRecord(c->step_b, c->stream));
     CK(cudaStreamSynchronize(c->stream));
     cudaEventElapsedTime(&c->last_step_ms, c->step_a, c->step_b);
-    RC(status_verdict(c, "kc_verify_step"));
+    RC(status_verdict(c, where));
     if (n_committed_out) memset(n_committed_out, 0, (size_t)n_seqs * 4);
     if (n_accepted_out) memset(n_accepted_out, 0, (size_t)n_seqs * 4);
   }
   return KC_OK;
+}
+
+extern "C" int kc_verify_step(kc_model_t m, kc_kv_t kv, const uint32_t* token_ids, int32_t n, const kc_seq_step* seqs,
+                              int32_t n_seqs, uint32_t* row_tokens_out, int32_t* n_committed_out, int32_t* n_accepted_out) {
+  return verify_round("kc_verify_step", m, kv, token_ids, n, seqs, n_seqs, nullptr, nullptr, row_tokens_out, nullptr, n_committed_out, n_accepted_out);
+}
+
+extern "C" int kc_verify_step_sampled(kc_model_t m, kc_kv_t kv, const uint32_t* token_ids, int32_t n, const kc_seq_step* seqs, int32_t n_seqs,
+                                      const kc_sampling* sampling, const float* uniform, uint32_t* row_tokens_out, float* logprobs_out,
+                                      int32_t* n_committed_out, int32_t* n_accepted_out) {
+  if (!sampling || !uniform) return fail(KC_ERR_INVALID, "kc_verify_step_sampled: NULL argument");
+  return verify_round("kc_verify_step_sampled", m, kv, token_ids, n, seqs, n_seqs, sampling, uniform, row_tokens_out, logprobs_out, n_committed_out,
+                      n_accepted_out);
 }
 
 extern "C" int kc_draft_chain(kc_model_t m, kc_kv_t kv, uint32_t first_token, int32_t offset, const uint32_t* blocks,

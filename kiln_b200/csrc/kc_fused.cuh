@@ -89,6 +89,13 @@ cudaError_t launch_copy_block(bf16* pool, int layers, int NB, size_t block_elems
 cudaError_t launch_greedy_rows(const bf16* logits, int rows, int vocab, int normalize, uint32_t* tokens,
                                cudaStream_t s, uint32_t* tokens_host = nullptr, const uint32_t* status = nullptr,
                                uint32_t* status_copy = nullptr);
+// A token drawn per logits row; see kc_sample_rows in kiln_cuda.h, whose kc_sampling a DrawSetting is. ld: values from row to row.
+// logprobs, tokens_host, logprobs_host (the last two in pinned host memory): optional. skip_greedy: rows of no temperature
+// are left as they are.
+struct alignas(16) DrawSetting { float temperature; int32_t top_k; float top_p, min_p; };
+cudaError_t launch_draw_rows(const bf16* logits, long long ld, int rows, int vocab, const DrawSetting* settings, const float* uniform,
+                             uint32_t* tokens, float* logprobs, int sm_count, cudaStream_t s, uint32_t* tokens_host = nullptr,
+                             float* logprobs_host = nullptr, int skip_greedy = 0);
 // tokens[i] = prev[feed[i]] where feed[i] >= 0: the device-side token feedback of kc_decode_launch.
 cudaError_t launch_feed_tokens(uint32_t* tokens, const int32_t* feed, const uint32_t* prev, int n, int prev_n, cudaStream_t s);
 // The settle walk per verify segment; see kc_verify_accept in kiln_cuda.h.
