@@ -243,17 +243,17 @@ class Context:
         return int(L.lib().kc_ctx_stream(self._h) or 0)
 
     def on_current_stream(self, call, *args) -> None:
-        """``call(handle, *args)``, an entry point that does not synchronise, as part of torch's current stream of this
+        """``call(*args)``, an entry point that does not synchronise, as part of torch's current stream of this
         context's device: behind what that stream and the context's hold, and ahead of what either is given later. The host
         waits for nothing, also in a capture into a graph. A program that makes the context's stream torch's current one
         (``torch.cuda.ExternalStream(ctx.stream)``) spares the two events that this takes."""
         current = torch.cuda.current_stream(self.device).cuda_stream
         if current == self._stream:
-            check(call(self._h, *args))
+            check(call(*args))
             return
         check(L.lib().kc_ctx_wait_stream(self._h, current))
         try:
-            check(call(self._h, *args))
+            check(call(*args))
         finally:
             check(L.lib().kc_stream_wait_ctx(self._h, current))
 
@@ -579,7 +579,7 @@ def sample_rows(ctx: Context, logits: torch.Tensor, params, uniforms: torch.Tens
             raise ValueError(f"{name}: contiguous {dtype} {list(shape)}")
     if any(t.device.type != "cuda" or t.device.index != ctx.device for t in (logits, params, uniforms, out, logprobs)):
         raise ValueError(f"tensors of a context on cuda:{ctx.device}")
-    ctx.on_current_stream(L.lib().kc_sample_rows, logits.data_ptr(), logits.stride(0), rows, vocab, params.data_ptr(), uniforms.data_ptr(),
+    ctx.on_current_stream(L.lib().kc_sample_rows, ctx._h, logits.data_ptr(), logits.stride(0), rows, vocab, params.data_ptr(), uniforms.data_ptr(),
                           out.data_ptr(), logprobs.data_ptr())
     return out, logprobs
 
@@ -686,6 +686,44 @@ def paged_attention(ctx: Context, kv: PagedKv, layer: int, q: torch.Tensor, seqs
     check(L.lib().kc_paged_attention(ctx._h, kv._h, layer, q.contiguous().data_ptr(), n, heads, p.seq_arr, p.n_seqs,
                                      scale, softcap, window, out.data_ptr()))   # returns when the work is done
     return out
+
+
+class AttentionPlan:
+    """The paged attention of one step, planned once and run for each layer (kc_attn_plan_create). Blocks at the start of the
+    tables that neighbouring sequences share are read once for all of them; a row has paged_attention's bits."""
+
+    def __init__(self, ctx: Context, kv: PagedKv, heads: int, seqs: Sequence[SeqStep]):
+        self.ctx, self.kv, self.heads = ctx, kv, heads
+        self._h = C.c_void_p()
+        self.tokens = sum(s.len for s in seqs)
+        p = _PackedStep(StepBatch([], seqs))
+        check(L.lib().kc_attn_plan_create(ctx._h, kv._h, p.seq_arr, p.n_seqs, heads, C.byref(self._h)))
+        ctx._adopt(self)
+
+    def run(self, layer: int, q: torch.Tensor, scale: float, softcap: float = 0.0, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q bf16 [tokens, heads, head_dim] post-RoPE → bf16 [tokens, heads*head_dim], part of torch's current stream
+        (Context.on_current_stream); the host does not wait. Runs of one plan come one after the other."""
+        if not self._h or not self.kv._h:
+            raise ValueError("the plan or its pools are closed")
+        dim = self.kv.spec.head_dim
+        if out is None:
+            out = torch.empty(self.tokens, self.heads * dim, dtype=torch.bfloat16, device=q.device)
+        for name, t, shape in (("q", q, (self.tokens, self.heads, dim)), ("out", out, (self.tokens, self.heads * dim))):
+            if t.dtype != torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device.type != "cuda" or t.device.index != self.ctx.device:
+                raise ValueError(f"{name}: contiguous bf16 {list(shape)} on cuda:{self.ctx.device}")
+        self.ctx.on_current_stream(L.lib().kc_attn_plan_run, self._h, layer, q.data_ptr(), scale, softcap, window, out.data_ptr())
+        return out
+
+    def close(self) -> None:
+        if self._h:
+            L.lib().kc_attn_plan_free(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def rope_kv_write(ctx: Context, kv: PagedKv, layer: int, qkv: torch.Tensor, inv_freq: torch.Tensor, heads: int,

@@ -161,7 +161,7 @@ struct Layer {
 
 // Per-step metadata, packed on the host and copied to the device in one transfer.
 struct MetaLayout {
-  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, sampling, uniform, total;
+  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, sampling, uniform, prefix_units, rest_units, total;
 };
 
 struct kc_model {
@@ -192,8 +192,10 @@ struct kc_model {
   float* argmax_scratch = nullptr;     // per-CTA bests + counter of the fused reduction / arg-max of a streamed head
   float* partial_gu = nullptr;         // gate_up's fp32 partials while a gated down projection reads them (stream lane on)
   float* attn_ws = nullptr; size_t attn_ws_bytes = 0;
-  CUtensorMap q_map, q_map_small;      // query maps of q_map_ptr [q_map_rows tokens], boxes of q_map_box and ATT_SMALL_TOKENS tokens
-  const void* q_map_ptr = nullptr; int q_map_box = 0, q_map_rows = 0, q_map_gqa = 0;
+  // Query maps of ptr [rows tokens], boxes of `box` and ATT_SMALL_TOKENS tokens: of a step's own units, and of the two launches of
+  // one that reads shared prefixes once.
+  struct QMaps { CUtensorMap map, small; const void* ptr = nullptr; int box = 0, rows = 0, gqa = 0; };
+  QMaps q_maps[3];
   float* tp_buf = nullptr;             // fp32 staging for the tensor-parallel all-reduce
   // Tensor-parallel exchange over peer memory (kc_tp_export / kc_tp_attach): the o_proj / down_proj output of exchange e
   // goes to tp_out[e & 1]; tp_flags[r] = the last exchange rank r has published. peer_* = every rank's buffers as
@@ -1088,6 +1090,14 @@ struct StepPlan {
   bool keys = false;               // attention by the kernel with a key per thread
   bool draws = false;              // sampled rows have settings and random numbers (kc_verify_step_sampled)
   std::vector<AttnUnit> units;
+  // The same attention with the chunks that neighbours share read once (plan_shared): units of those chunks over the rows of all
+  // that share them, and units of the other chunks. One launch of all units, in `rest`, where one kernel takes both.
+  struct Shared {
+    bool on = false;
+    std::vector<AttnUnit> prefix, rest;
+    int prefix_tokens = 1, rest_tokens = 1;   // of an item
+    bool prefix_keys = false, rest_keys = false;
+  } shared;
   MetaLayout lay{};
 };
 
@@ -1156,8 +1166,75 @@ std::vector<int> old_keys(kc_kv* kv, const kc_seq_step* seqs, int n_seqs) {
   return old;
 }
 
+// Units over shared prefixes. Sequences that stand next to each other in the step and name the same blocks for a chunk, and for
+// all chunks ahead of it, are a run there; no key of the chunk is written by the step. The run's rows are taken together against
+// the chunk, as many as a unit holds, and every chunk's partial result is merged in index order as ever: a row has the bits
+// that it has alone.
+void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& old, int block_size, int head_dim, int gqa, int kv_heads, int sm_count,
+                 bool alone, bool capped) {
+  StepPlan::Shared& sh = p->shared;
+  const int n = p->n_seqs, per = ATT_CHUNK / block_size;
+  std::vector<int> common(n + 1, 0), row(n + 1, 0);   // chunks that a sequence shares with the one before it; first row
+  int most = 0;
+  for (int i = 0; i < n; ++i) {
+    row[i + 1] = row[i] + seqs[i].len;
+    if (i == 0) continue;
+    const int limit = std::min(old[i - 1], old[i]) / ATT_CHUNK;
+    int& c = common[i];
+    while (c < limit && std::equal(seqs[i].blocks + c * per, seqs[i].blocks + (c + 1) * per, seqs[i - 1].blocks + c * per)) ++c;
+    most = std::max(most, c);
+  }
+  if (most == 0) return;
+  int widest = 1;   // tokens of a run
+  long long rest_tiles = 0;
+  auto runs = [&](int c, auto&& each) {
+    for (int i = 0, j; i < n; i = j + 1) {
+      for (j = i; j + 1 < n && common[j + 1] > c; ++j) {}
+      if (j > i) each(i, row[i], row[j + 1]);
+    }
+  };
+  runs(0, [&](int, int r0, int r1) { widest = std::max(widest, r1 - r0); });
+  for (int i = 0; i < n; ++i) rest_tiles += (seqs[i].offset + seqs[i].len - std::max(common[i], common[i + 1]) * ATT_CHUNK + 127) / 128;
+  sh.rest_tokens = p->tokens_per_item;
+  sh.rest_keys = sh.rest_tokens * gqa <= attn_key_rows(head_dim, alone, capped, AttnForm::apart, rest_tiles * kv_heads, sm_count);
+  sh.prefix_keys = widest * gqa <= KEY_ROWS;
+  sh.prefix_tokens = std::min(std::max(1, (sh.prefix_keys ? KEY_ROWS : ATT_ROWS) / gqa), widest);
+  auto small = [](int box, int tokens) { return box > ATT_SMALL_TOKENS && tokens <= ATT_SMALL_TOKENS ? 1 : 0; };
+  const bool one_launch = sh.prefix_keys == sh.rest_keys;
+  if (one_launch) sh.prefix_tokens = sh.rest_tokens = std::max(sh.prefix_tokens, sh.rest_tokens);
+  for (int c = 0; c < most; ++c)
+    runs(c, [&](int i, int r0, int r1) {
+      for (int t = r0; t < r1; t += sh.prefix_tokens) {
+        AttnUnit u{};
+        u.seq = i; u.tok0 = t; u.ntok = std::min(sh.prefix_tokens, r1 - t);
+        u.pos0 = u.old = (c + 1) * ATT_CHUNK;   // every row lies past the chunk
+        u.chunk0 = c; u.chunk1 = c + 1;
+        u.small = small(sh.prefix_tokens, u.ntok);
+        sh.prefix.push_back(u);
+      }
+    });
+  std::vector<AttnUnit> full, last;
+  for (int i = 0; i < n; ++i)
+    for (int t = 0; t < seqs[i].len; t += p->tokens_per_item) {
+      AttnUnit u{};
+      u.seq = i; u.tok0 = row[i] + t; u.ntok = std::min(p->tokens_per_item, seqs[i].len - t); u.pos0 = seqs[i].offset + t;
+      u.small = small(sh.rest_tokens, u.ntok);
+      u.old = old[i];
+      const int end = (u.pos0 + u.ntok - 1) / ATT_CHUNK + 1;
+      for (int c = std::max(common[i], common[i + 1]); c < end; ++c) {
+        u.chunk0 = c; u.chunk1 = c + 1;
+        (c + 1 < end ? full : last).push_back(u);
+      }
+    }
+  std::stable_sort(last.begin(), last.end(), [](const AttnUnit& a, const AttnUnit& b) { return (a.pos0 + a.ntok - 1) % ATT_CHUNK > (b.pos0 + b.ntok - 1) % ATT_CHUNK; });
+  if (one_launch) sh.rest.swap(sh.prefix);
+  sh.rest.insert(sh.rest.end(), full.begin(), full.end());
+  sh.rest.insert(sh.rest.end(), last.begin(), last.end());
+  sh.on = true;
+}
+
 int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, const kc_seq_step* seqs, int32_t n_seqs,
-                  int32_t pad_rows, StepPlan* plan, bool alone = false, bool capped = false, bool draws = false) {
+                  int32_t pad_rows, StepPlan* plan, bool alone = false, bool capped = false, bool draws = false, bool share = false) {
   if (!m || !kv || !token_ids || !seqs) return fail(KC_ERR_INVALID, "forward_step: NULL argument");
   if (kv->ctx != m->ctx) return fail(KC_ERR_INVALID, "forward_step: model and pools belong to different contexts");
   if (kv->layers != m->d.num_layers || kv->kv_heads != m->Hkv || kv->head_dim != m->d.head_dim)
@@ -1194,7 +1271,9 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
   const int gqa = m->d.num_heads / m->d.num_kv_heads;
   p.tokens_per_item = attn_tokens_per_item(gqa, p.max_len);
   p.max_chunks = (max_ctx + ATT_CHUNK - 1) / ATT_CHUNK;
-  plan_attention(&p, seqs, old_keys(kv, seqs, n_seqs), m->d.head_dim, gqa, m->Hkv, m->ctx->sm_count, alone, capped);
+  const std::vector<int> old = old_keys(kv, seqs, n_seqs);
+  plan_attention(&p, seqs, old, m->d.head_dim, gqa, m->Hkv, m->ctx->sm_count, alone, capped);
+  if (share) plan_shared(&p, seqs, old, kv->block_size, m->d.head_dim, gqa, m->Hkv, m->ctx->sm_count, alone, capped);
   MetaLayout& L = p.lay;
   size_t at = 0;
   auto put = [&](size_t bytes) { size_t o = at; at = align_up(at + bytes, 16); return o; };
@@ -1206,6 +1285,7 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
   L.v_draft = put((size_t)n * 4);
   L.feed = put((size_t)n * 4);
   if (p.draws) { L.sampling = put((size_t)p.n_sampled * sizeof(kc_sampling)); L.uniform = put((size_t)p.n_sampled * 4); }
+  if (p.shared.on) { L.prefix_units = put(p.shared.prefix.size() * sizeof(AttnUnit)); L.rest_units = put(p.shared.rest.size() * sizeof(AttnUnit)); }
   L.total = at;
   *plan = std::move(p);
   return KC_OK;
@@ -1238,7 +1318,10 @@ int upload_meta(kc_model* m, kc_kv* kv, const uint32_t* token_ids, const kc_seq_
   int32_t* slotv = reinterpret_cast<int32_t*>(hbuf + L.kv_slot);
   int32_t* sampled = reinterpret_cast<int32_t*>(hbuf + L.sampled);
   int32_t* tables = reinterpret_cast<int32_t*>(hbuf + L.tables);
-  memcpy(hbuf + L.units, p.units.data(), p.units.size() * sizeof(AttnUnit));
+  auto put_units = [&](size_t to, const std::vector<AttnUnit>& u) { if (!u.empty()) memcpy(hbuf + to, u.data(), u.size() * sizeof(AttnUnit)); };
+  put_units(L.units, p.units);
+  put_units(L.prefix_units, p.shared.prefix);
+  put_units(L.rest_units, p.shared.rest);
   int32_t* v_row = reinterpret_cast<int32_t*>(hbuf + L.v_row_off);
   int32_t* v_doff = reinterpret_cast<int32_t*>(hbuf + L.v_draft_off);
   int32_t* v_dlen = reinterpret_cast<int32_t*>(hbuf + L.v_draft_len);
@@ -1274,7 +1357,7 @@ int upload_meta(kc_model* m, kc_kv* kv, const uint32_t* token_ids, const kc_seq_
 }
 
 int ensure_attn_ws(kc_model* m, const StepPlan& p) {
-  if (p.whole) return KC_OK;   // no partials
+  if (p.whole && !p.shared.on) return KC_OK;   // no partials
   const size_t rows = (size_t)p.n * m->Hq * p.max_chunks;
   const size_t need = rows * m->d.head_dim * 4 + rows * 8 + 256;
   if (need > m->attn_ws_bytes) {
@@ -1304,24 +1387,52 @@ AttnParams attn_params(kc_model* m, kc_kv* kv, const StepPlan& p, int layer, bf1
   a.Hq = Hq; a.Hkv = kv->kv_heads; a.gqa = Hq / kv->kv_heads;
   a.layer = layer; a.NB = kv->num_blocks; a.BS = kv->block_size;
   a.max_chunks = p.max_chunks;
-  a.whole = p.whole ? 1 : 0; a.single = p.max_chunks == 1 ? 1 : 0; a.keys = p.keys ? 1 : 0;
+  a.whole = p.whole ? 1 : 0; a.single = p.max_chunks == 1 ? 1 : 0; a.keys = p.keys ? 1 : 0; a.merge = 1;
   a.scale = scale; a.softcap = softcap; a.window = window;
   a.q_tokens = p.tokens_per_item;
   a.kv5d = kv->map5d ? 1 : 0;
   return a;
 }
-// Kernels one attention call of this plan launches.
-int attn_launches(const StepPlan& p) { return p.whole || p.max_chunks == 1 ? 1 : 2; }
-
 // The query maps of a buffer of `rows` tokens: encoded again only when the buffer or a step's item size changes.
-int ensure_q_maps(kc_model* m, const bf16* q, int rows, int Hq, int gqa, const StepPlan& p) {
-  if (m->q_map_ptr == q && m->q_map_rows == rows && m->q_map_box == p.tokens_per_item && m->q_map_gqa == gqa) return KC_OK;
+int ensure_q_map(kc_model* m, kc_model::QMaps* q, const bf16* ptr, int rows, int Hq, int gqa, int box) {
+  if (q->ptr == ptr && q->rows == rows && q->box == box && q->gqa == gqa) return KC_OK;
   const char* err = "";
-  const int D = m->d.head_dim, small = std::min(p.tokens_per_item, ATT_SMALL_TOKENS);
-  if (!make_tmap_q(&m->q_map, q, rows, Hq, gqa, D, p.tokens_per_item, &err) || !make_tmap_q(&m->q_map_small, q, rows, Hq, gqa, D, small, &err))
+  const int D = m->d.head_dim, small = std::min(box, ATT_SMALL_TOKENS);
+  q->ptr = nullptr;
+  if (!make_tmap_q(&q->map, ptr, rows, Hq, gqa, D, box, &err) || !make_tmap_q(&q->small, ptr, rows, Hq, gqa, D, small, &err))
     return fail(KC_ERR_CUDA, "attention queries: %s", err);
-  m->q_map_ptr = q; m->q_map_rows = rows; m->q_map_box = p.tokens_per_item; m->q_map_gqa = gqa;
+  q->ptr = ptr; q->rows = rows; q->box = box; q->gqa = gqa;
   return KC_OK;
+}
+int ensure_q_maps(kc_model* m, const bf16* q, int rows, int Hq, int gqa, const StepPlan& p) {
+  RC(ensure_q_map(m, &m->q_maps[0], q, rows, Hq, gqa, p.tokens_per_item));
+  if (!p.shared.on) return KC_OK;
+  RC(ensure_q_map(m, &m->q_maps[1], q, rows, Hq, gqa, p.shared.rest_tokens));
+  return p.shared.prefix.empty() ? KC_OK : ensure_q_map(m, &m->q_maps[2], q, rows, Hq, gqa, p.shared.prefix_tokens);
+}
+
+// One layer's attention of a step whose maps and workspace are there. Every row of a windowed layer has a mask of its own, so
+// those take the step's own units.
+int run_attention(kc_model* m, kc_kv* kv, const StepPlan& p, int layer, bf16* out, float scale, float softcap, int window, int Hq, bool in_order) {
+  kc_ctx* c = m->ctx;
+  AttnParams a = attn_params(m, kv, p, layer, out, scale, softcap, window, Hq);
+  auto launch = [&](const kc_model::QMaps& q, int launches, bool ordered) -> int {
+    LAUNCH(c, KC_PROF_ATTN, launches, paged_attention(kv->map, kv->map_one, q.map, q.small, a, ordered, kv->head_dim, p.n, c->sm_count, c->stream));
+    return KC_OK;
+  };
+  if (!p.shared.on || window > 0) return launch(m->q_maps[0], p.whole || p.max_chunks == 1 ? 1 : 2, in_order);
+  a.whole = a.single = 0;
+  const bool two = !p.shared.prefix.empty();
+  if (two) {
+    a.units = reinterpret_cast<const AttnUnit*>(m->meta_dev + p.lay.prefix_units);
+    a.n_units = (int)p.shared.prefix.size();
+    a.q_tokens = p.shared.prefix_tokens; a.keys = p.shared.prefix_keys ? 1 : 0; a.merge = 0;
+    RC(launch(m->q_maps[2], 1, in_order));
+  }
+  a.units = reinterpret_cast<const AttnUnit*>(m->meta_dev + p.lay.rest_units);
+  a.n_units = (int)p.shared.rest.size();
+  a.q_tokens = p.shared.rest_tokens; a.keys = p.shared.rest_keys ? 1 : 0; a.merge = 1;
+  return launch(m->q_maps[1], 2, in_order && !two);
 }
 
 // Brings every tensor-parallel rank's bf16 [n, H] sublayer output to every rank: out[r] = rank r's rows. The SUM is
@@ -1409,8 +1520,7 @@ int run_forward(kc_model* m, kc_kv* kv, const uint32_t* tokens_dev, const StepPl
     LAUNCH(c, KC_PROF_ROWWISE, 1, launch_rope_kv_write(so, L.qkv_bias, m->inv_freq, token_pos, kv_slot, n, m->Hq, m->Hkv, D, d.rope_traditional, l,
                             kv->num_blocks, kv->block_size, kv->pool, m->q_rot, c->stream));
     const int window = (d.sliding_window > 0 && (l % 2 == 0)) ? d.sliding_window : 0;
-    AttnParams a = attn_params(m, kv, p, l, m->attn, m->attn_scale, gemma ? d.attn_logit_softcapping : 0.f, window, m->Hq);
-    LAUNCH(c, KC_PROF_ATTN, attn_launches(p), paged_attention(kv->map, kv->map_one, m->q_map, m->q_map_small, a, false, D, n, c->sm_count, c->stream));
+    RC(run_attention(m, kv, p, l, m->attn, m->attn_scale, gemma ? d.attn_logit_softcapping : 0.f, window, m->Hq, false));
     if (streams(L.o)) RC(run_stream(c, L.o, m->attn, n, m->proj, H, m->partial, &so));
     else if (small(L.o)) RC(run_gemv(c, L.o, m->attn, n, m->proj, H, m->partial, &so));
     else RC(run_qlinear(c, L.o, m->op_attn, n, d.tp_world > 1 ? tp_out_buffer(m) : m->proj, H, m->partial, d.tp_world > 1 ? nullptr : &so));
@@ -1766,21 +1876,25 @@ extern "C" int kc_decode_collect(kc_model_t m, uint64_t ticket, uint32_t* row_to
 // call made it grow to is given back at the end of that call (op_shell_done); a context is used from one host thread.
 constexpr size_t OP_KEEP_BYTES = (size_t)64 << 20;
 
-static int op_shell(kc_ctx* c, kc_kv* kv, int num_heads, int n, int n_seqs, kc_model** out) {
-  if (!c->op) {
-    kc_model* s = new kc_model;
-    s->ctx = c;
-    for (int i = 0; i < kc_model::kStaging; ++i)
-      if (cudaEventCreateWithFlags(&s->meta_ev[i], cudaEventDisableTiming) != cudaSuccess) { free_model(s); return fail(KC_ERR_CUDA, "event"); }
-    c->op = s;
-  }
-  kc_model* m = c->op;
+static int new_shell(kc_ctx* c, kc_model** out) {
+  kc_model* s = new kc_model;
+  s->ctx = c; s->device = c->device;
+  for (int i = 0; i < kc_model::kStaging; ++i)
+    if (cudaEventCreateWithFlags(&s->meta_ev[i], cudaEventDisableTiming) != cudaSuccess) { free_model(s); return fail(KC_ERR_CUDA, "event"); }
+  *out = s;
+  return KC_OK;
+}
+static void set_shell(kc_model* m, kc_kv* kv, int num_heads, int n, int n_seqs) {
   m->d.num_layers = kv->layers; m->d.head_dim = kv->head_dim; m->d.num_heads = num_heads; m->d.num_kv_heads = kv->kv_heads;
   m->d.vocab_size = 0x7fffffff; m->d.hidden_size = 0; m->d.max_step_tokens = n; m->d.tp_world = 1;
-  m->q_map_ptr = nullptr;   // head counts and head size may differ from the last call's
+  for (auto& q : m->q_maps) q.ptr = nullptr;   // head counts and head size may differ from the last call's
   m->Hq = num_heads; m->Hkv = kv->kv_heads;
   m->max_rows = n; m->max_seqs = n_seqs; m->logit_rows = n;
-  *out = m;
+}
+static int op_shell(kc_ctx* c, kc_kv* kv, int num_heads, int n, int n_seqs, kc_model** out) {
+  if (!c->op) RC(new_shell(c, &c->op));
+  set_shell(c->op, kv, num_heads, n, n_seqs);
+  *out = c->op;
   return KC_OK;
 }
 static void free_op_shell(kc_ctx* c) {
@@ -1825,9 +1939,8 @@ extern "C" int kc_paged_attention(kc_ctx_t c, kc_kv_t kv, int32_t layer, const v
     if (e != cudaSuccess) { out = (bf16*)out_dev; rc = fail(KC_ERR_OOM, "kc_paged_attention: %zu bytes: %s", out_bytes, cudaGetErrorString(e)); }
   }
   if (!rc) {
-    AttnParams a = attn_params(m, kv, p, layer, out, scale, softcap, window, num_heads);
     rc = [&]() -> int {
-      LAUNCH(c, KC_PROF_ATTN, attn_launches(p), paged_attention(kv->map, kv->map_one, m->q_map, m->q_map_small, a, true, kv->head_dim, n, c->sm_count, c->stream));
+      RC(run_attention(m, kv, p, layer, out, scale, softcap, window, num_heads, true));
       if (out != out_dev) CK(cudaMemcpyAsync(out_dev, out, out_bytes, cudaMemcpyDeviceToDevice, c->stream));
       return KC_OK;
     }();
@@ -1835,6 +1948,73 @@ extern "C" int kc_paged_attention(kc_ctx_t c, kc_kv_t kv, int32_t layer, const v
   rc = op_shell_done(c, rc, "kc_paged_attention");
   if (out != out_dev) cudaFree(out);
   return rc;
+}
+
+// A step's attention kept as a handle: its metadata and workspace in a shell of its own, for softcap off and on (which kernel is the
+// faster one hangs on that).
+struct kc_attn_plan {
+  kc_ctx* ctx = nullptr;
+  kc_kv* kv = nullptr;
+  int device = 0, num_heads = 0;
+  kc_model* shell[2] = {nullptr, nullptr};
+  StepPlan plan[2];
+};
+static void free_attn_plan(kc_attn_plan* p) {
+  for (kc_model* m : p->shell) if (m) free_model(m);
+  delete p;
+}
+
+extern "C" int kc_attn_plan_create(kc_ctx_t c, kc_kv_t kv, const kc_seq_step* seqs, int32_t n_seqs, int32_t num_heads, kc_attn_plan_t* out) {
+  if (!c || !kv || !seqs || !out) return fail(KC_ERR_INVALID, "kc_attn_plan_create: NULL argument");
+  if (kv->ctx != c) return fail(KC_ERR_INVALID, "kc_attn_plan_create: the pools belong to another context");
+  if (num_heads < kv->kv_heads || num_heads % kv->kv_heads || num_heads / kv->kv_heads > 64)
+    return fail(KC_ERR_INVALID, "kc_attn_plan_create: %d heads over %d kv heads", num_heads, kv->kv_heads);
+  long long n = 0;
+  for (int i = 0; i < n_seqs; ++i) n += std::max(0, seqs[i].len);
+  if (n_seqs < 1 || n < 1 || n > 1 << 24) return fail(KC_ERR_INVALID, "kc_attn_plan_create: %lld token(s) of %d sequence(s)", n, n_seqs);
+  OnDevice on;
+  CK(on.enter(c->device));
+  kc_attn_plan* p = new kc_attn_plan;
+  p->ctx = c; p->kv = kv; p->device = c->device; p->num_heads = num_heads;
+  std::vector<uint32_t> ids((size_t)n, 0);
+  int rc = KC_OK;
+  for (int capped = 0; capped < 2 && !rc; ++capped) {
+    kc_model* m = nullptr;
+    rc = new_shell(c, &m);
+    p->shell[capped] = m;
+    if (rc) break;
+    set_shell(m, kv, num_heads, (int)n, n_seqs);
+    rc = validate_step(m, kv, ids.data(), (int32_t)n, seqs, n_seqs, 0, &p->plan[capped], true, capped != 0, false, true);
+    if (!rc) rc = upload_meta(m, kv, ids.data(), seqs, p->plan[capped]);
+    if (!rc) rc = ensure_attn_ws(m, p->plan[capped]);
+  }
+  if (!rc && cudaStreamSynchronize(c->stream) != cudaSuccess) rc = fail(KC_ERR_CUDA, "kc_attn_plan_create: the copy of the plan failed");
+  if (rc) { std::string keep = g_err; free_attn_plan(p); g_err = keep; return rc; }
+  g_live++;
+  *out = p;
+  return KC_OK;
+}
+
+extern "C" void kc_attn_plan_free(kc_attn_plan_t p) {
+  if (!p) return;
+  OnDevice on;
+  on.enter(p->device);
+  quiesce(p->ctx, p->device);
+  free_attn_plan(p);
+  g_live--;
+}
+
+extern "C" int kc_attn_plan_run(kc_attn_plan_t p, int32_t layer, const void* q_dev, float scale, float softcap, int32_t window, void* out_dev) {
+  if (!p || !q_dev || !out_dev) return fail(KC_ERR_INVALID, "kc_attn_plan_run: NULL argument");
+  if (layer < 0 || layer >= p->kv->layers) return fail(KC_ERR_INVALID, "kc_attn_plan_run: layer %d of %d", layer, p->kv->layers);
+  if ((uintptr_t)q_dev % 16 || (uintptr_t)out_dev % 16) return fail(KC_ERR_INVALID, "kc_attn_plan_run: q and out must be 16-byte aligned");
+  OnDevice on;
+  CK(on.enter(p->device));
+  const int capped = softcap > 0.f ? 1 : 0;
+  kc_model* m = p->shell[capped];
+  const StepPlan& plan = p->plan[capped];
+  RC(ensure_q_maps(m, (const bf16*)q_dev, plan.n, p->num_heads, p->num_heads / p->kv->kv_heads, plan));
+  return run_attention(m, p->kv, plan, layer, (bf16*)out_dev, scale, softcap, window, p->num_heads, true);
 }
 
 extern "C" int kc_rope_kv_write(kc_ctx_t c, kc_kv_t kv, int32_t layer, const void* qkv_dev, const void* qkv_bias_dev,

@@ -1,0 +1,222 @@
+"""Attention of sequences that share a prefix: the bits of paged_attention for every row, whatever is shared by whom, and the
+formula in 64 bits. Against that the 2-norm of the error is that of rounding the output to bf16 (half a step, 2^-9 of a value
+at the most: 1.7e-3 of the norm on the average of mantissas) and of its fp32 parts, far below."""
+import numpy as np
+import pytest
+import torch
+
+from kiln_b200 import api
+from kiln_b200.synth import PRESETS, synth_checkpoint
+
+pytestmark = pytest.mark.gpu
+
+
+def pools(ctx, kv_heads, dim, blocks, block_size, seed, layers=1, std=1.0):
+    """Random K and V, written through rope_kv_write without a rotation: (PagedKv, [layers, 2, blocks, kv heads, block, dim])."""
+    kv = api.PagedKv(ctx, api.KvSpec(layers, kv_heads, dim, blocks, block_size))
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    data = torch.empty(layers, 2, blocks, kv_heads, block_size, dim, device="cuda").normal_(0, std, generator=g).to(torch.bfloat16)
+    for layer in range(layers):
+        k, v = (t.transpose(1, 2).reshape(-1, kv_heads * dim) for t in data[layer])
+        seq = api.SeqStep(blocks * block_size, 0, 0, np.arange(blocks, dtype=np.uint32))
+        api.rope_kv_write(ctx, kv, layer, torch.cat([k, k, v], 1), torch.zeros(dim // 2, device="cuda"), kv_heads, [seq])
+    return kv, data
+
+
+def tables(groups, block_size, seed):
+    """groups: [(shared tokens, [(len, offset), ..]), ..] -> SeqSteps over permuted blocks, and the number of blocks. The first
+    shared // block_size blocks of a group's tables are the same."""
+    want = []
+    for shared, members in groups:
+        first = shared // block_size
+        want.append((first, [(ln, off, -(-(ln + off) // block_size)) for ln, off in members]))
+    total = sum(f + sum(n - f for _, _, n in m) for f, m in want)
+    order, at, seqs = np.random.default_rng(seed).permutation(total), 0, []
+    for first, members in want:
+        head = order[at: at + first]
+        at += first
+        for ln, off, n in members:
+            seqs.append(api.SeqStep(ln, off, 0, np.concatenate([head, order[at: at + n - first]]).astype(np.uint32)))
+            at += n - first
+    return seqs, total
+
+
+def formula(data, q, seqs, scale, softcap):
+    hkv, dim, rows = data.shape[2], data.shape[4], []
+    at = 0
+    for s in seqs:
+        k, v = (t[torch.from_numpy(s.blocks.astype(np.int64)).cuda()].transpose(1, 2).reshape(-1, hkv, dim).double() for t in data)
+        for r in range(s.len):
+            n = s.offset + r + 1
+            x = q[at].double().view(hkv, -1, dim)
+            a = torch.einsum("hgd,khd->hgk", x, k[:n]) * scale
+            if softcap:
+                a = softcap * torch.tanh(a / softcap)
+            rows.append(torch.einsum("hgk,khd->hgd", torch.softmax(a, -1), v[:n]).reshape(-1))
+            at += 1
+    return torch.stack(rows)
+
+
+def close(out, want):
+    assert float((out.double() - want).norm() / want.norm()) < 2.0e-3
+    assert float((out.double() - want).abs().max()) <= 2 ** -8 * float(want.abs().max())
+
+
+def run_both(ctx, kv, data, heads, seqs, seed, softcap=0.0, scale=None, layer=0, std=1.5):
+    n, dim = sum(s.len for s in seqs), data.shape[-1]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.empty(n, heads, dim, device="cuda").normal_(0, std, generator=g).to(torch.bfloat16)
+    scale = dim ** -0.5 if scale is None else scale
+    plan = api.AttentionPlan(ctx, kv, heads, seqs)
+    got = plan.run(layer, q, scale, softcap)
+    torch.cuda.synchronize()
+    want = api.paged_attention(ctx, kv, layer, q, seqs, scale, softcap)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+    return q, got, plan
+
+
+HEADS = [(32, 8, 128), (28, 4, 128), (32, 8, 64), (16, 8, 256), (8, 8, 128), (24, 1, 64), (64, 1, 128)]
+SHARED = {
+    "two of one chunk": [(512, [(1, 512), (1, 600)])],
+    "one chunk, ends on its edge": [(512, [(1, 511), (1, 512), (1, 513)])],       # the first one's own row stands in the chunk: not shared with it
+    "not a block's multiple": [(1001, [(1, 1001), (1, 1030), (1, 1500)])],
+    "verify rows": [(1024, [(5, 1300)] * 9)],
+    "ragged rows": [(1536, [(3, 1600), (1, 1536), (6, 2100), (2, 1700), (40, 1550)])],
+    "many": [(1100, [(1, 1100 + 7 * i) for i in range(70)])],
+    "two groups and loners": [(0, [(1, 700)]), (1024, [(1, 1100), (2, 1024)]), (0, [(1, 3), (1, 0)]), (2048, [(1, 2050), (1, 3000), (1, 2048)])],
+    "nothing shared": [(0, [(1, 900), (1, 800)])],
+    "shared below a chunk": [(496, [(1, 900), (1, 800)])],
+    "alone": [(2000, [(4, 2040)])],
+    "no history": [(0, [(1, 0)])],
+    "a piece of a prompt behind a shared prefix": [(1024, [(130, 1024), (1, 1200), (1, 1300)])],
+}
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("name", list(SHARED))
+def test_rows_have_the_bits_that_they_have_alone(ctx, heads, kv_heads, dim, name):
+    seqs, total = tables(SHARED[name], 16, len(name))
+    kv, data = pools(ctx, kv_heads, dim, total, 16, 5)
+    softcap = 30.0 if dim == 256 else 0.0
+    q, got, _ = run_both(ctx, kv, data, heads, seqs, 7, softcap)
+    close(got, formula(data[0], q, seqs, dim ** -0.5, softcap))
+    assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("block_size", [16, 32, 64, 128])
+@pytest.mark.parametrize("softcap,scale", [(0.0, None), (20.0, None), (0.0, -0.1), (0.0, 0.0), (5.0, 3.0)])
+def test_block_sizes_caps_and_scales(ctx, block_size, softcap, scale):
+    seqs, total = tables([(1024, [(2, 1100 + 130 * i) for i in range(6)])], block_size, 3)
+    kv, data = pools(ctx, 2, 128, total, block_size, 9)
+    run_both(ctx, kv, data, 8, seqs, 1, softcap, scale)
+
+
+def test_a_tree_of_prefixes(ctx):
+    """All share a chunk, pairs three, and the middle ones another two: every chunk goes by who has it in common."""
+    bs, rng = 16, np.random.default_rng(2)
+    per, order = 32, np.random.default_rng(2).permutation(2000)
+    trunk, branches, at, seqs = order[:per], [order[per * (1 + 2 * i): per * (3 + 2 * i)] for i in range(4)], 1000, []
+    deeper = order[per * 10: per * 12]
+    for i in range(8):
+        off = 512 + 1024 + (1024 if i in (3, 4, 5) else 0) + int(rng.integers(0, 300))
+        head = [trunk, branches[i // 2]] + ([deeper] if i in (3, 4, 5) else [])
+        head = np.concatenate(head)
+        n = -(-(off + 1 + i % 3) // bs)
+        own = order[at: at + n - len(head)]
+        at += len(own)
+        seqs.append(api.SeqStep(1 + i % 3, off, 0, np.concatenate([head, own]).astype(np.uint32)))
+    kv, data = pools(ctx, 4, 128, 2000, bs, 4)
+    q, got, _ = run_both(ctx, kv, data, 16, seqs, 3)
+    close(got, formula(data[0], q, seqs, 128 ** -0.5, 0.0))
+
+
+def test_one_table_for_all(ctx):
+    """Every block is shared, the rows' own among them, at different positions."""
+    kv, data = pools(ctx, 2, 128, 80, 16, 4)
+    table = np.random.default_rng(0).permutation(80).astype(np.uint32)
+    seqs = [api.SeqStep(3, off, 0, table) for off in (1000, 1024, 1100, 40, 600, 1277)]
+    q, got, _ = run_both(ctx, kv, data, 8, seqs, 3)
+    close(got, formula(data[0], q, seqs, 128 ** -0.5, 0.0))
+
+
+def test_windows_layers_streams_and_graphs(ctx):
+    """A plan serves all layers, windowed ones too, on whatever stream is the current one, and in a graph that is replayed after
+    the queries and the pools have changed."""
+    seqs, total = tables([(1024, [(2, 1030 + 50 * i) for i in range(7)])], 16, 1)
+    kv, data = pools(ctx, 2, 128, total, 16, 4, layers=2)
+    q, got, plan = run_both(ctx, kv, data, 8, seqs, 3, layer=1)
+    scale = 128 ** -0.5
+    for window in (1, 100, 600, 5000):
+        w = plan.run(0, q, scale, 0.0, window)
+        torch.cuda.synchronize()
+        assert torch.equal(w, api.paged_attention(ctx, kv, 0, q, seqs, scale, 0.0, window))
+    for stream in (torch.cuda.Stream(), torch.cuda.ExternalStream(ctx.stream)):
+        with torch.cuda.stream(stream):
+            x = torch.zeros_like(q)
+            for _ in range(10):
+                x.copy_(q)
+                a = plan.run(1, x, scale)
+                x.zero_()
+        torch.cuda.synchronize()
+        assert torch.equal(a, got)
+    still, out = q.clone(), torch.empty_like(got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run(0, still, scale, out=out)
+        plan.run(1, still, scale, 10.0)
+    ctx.sync()
+    for turn in range(2):
+        still.copy_(q if turn else -q)
+        kv.copy_block(int(seqs[0].blocks[turn]), int(seqs[0].blocks[3]))
+        ctx.sync()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, api.paged_attention(ctx, kv, 0, still, seqs, scale))
+    assert ctx.device_status() == 0
+
+
+def test_large_scores(ctx):
+    """One key outweighs all others by far: maxima that move by thousands of binary orders from chunk to chunk."""
+    seqs, total = tables([(512, [(1, 520), (1, 700), (2, 512)])], 16, 1)
+    kv, data = pools(ctx, 2, 64, total, 16, 4, std=40.0)
+    q, got, _ = run_both(ctx, kv, data, 8, seqs, 3, std=40.0)
+    close(got, formula(data[0], q, seqs, 64 ** -0.5, 0.0))
+
+
+def test_rows_past_the_shared_ones_are_left(ctx):
+    seqs, total = tables([(512, [(1, 512)] * 3)], 16, 1)
+    kv, data = pools(ctx, 2, 64, total, 16, 4)
+    q = torch.randn(3, 8, 64, device="cuda").to(torch.bfloat16)
+    out = torch.full((5, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    api.AttentionPlan(ctx, kv, 8, seqs).run(0, q, 0.125, out=out[1:4])
+    torch.cuda.synchronize()
+    assert (out[0] == 7).all() and (out[4] == 7).all() and torch.equal(out[1:4], api.paged_attention(ctx, kv, 0, q, seqs, 0.125))
+
+
+def test_refusals(ctx):
+    live = api.live_objects()
+    kv, _ = pools(ctx, 2, 64, 40, 16, 4)
+    good = [api.SeqStep(1, 20, 0, np.arange(4, dtype=np.uint32))]
+    for heads, seqs in ((3, good), (0, good), (2 * 65, good), (8, []), (8, [api.SeqStep(0, 3, 0, good[0].blocks)]), (8, [api.SeqStep(1, -1, 0, good[0].blocks)]),
+                        (8, [api.SeqStep(1, 64, 0, good[0].blocks)]), (8, [api.SeqStep(1, 3, 0, np.array([40], dtype=np.uint32))])):
+        with pytest.raises(api.KcError):
+            api.AttentionPlan(ctx, kv, heads, seqs)
+    plan = api.AttentionPlan(ctx, kv, 8, good)
+    q = torch.zeros(1, 8, 64, dtype=torch.bfloat16, device="cuda")
+    for bad in (q.float(), q[:, :4], q.expand(2, 8, 64), q.cpu(), torch.zeros(1, 8, 128, dtype=torch.bfloat16, device="cuda")[:, :, ::2]):
+        with pytest.raises(ValueError):
+            plan.run(0, bad, 1.0)
+    for layer in (-1, 1):
+        with pytest.raises(api.KcError):
+            plan.run(layer, q, 1.0)
+    with pytest.raises(api.KcError):
+        plan.run(0, torch.zeros(513, dtype=torch.bfloat16, device="cuda")[1:].view(1, 8, 64), 1.0)
+    plan.run(0, q, 1.0)
+    ctx.sync()
+    kv.close()
+    with pytest.raises(ValueError):
+        plan.run(0, q, 1.0)
+    plan.close()
+    with pytest.raises(ValueError):
+        plan.run(0, q, 1.0)
+    assert api.live_objects() == live
