@@ -396,6 +396,29 @@ KC_API int kc_quantized_matmul_static(kc_ctx_t ctx, kc_qweight_t w, const void* 
 /* Size of that array in bytes (a compile-time constant of the library). */
 KC_API int64_t kc_static_scratch_bytes(void);
 
+/* Low-rank adapters of many requests beside one projection (no counterpart in the reference): out_i = y_i + scale_a B_a (A_a x_i)
+ * for every row i, a being the adapter of its request; rows without one keep their y. A x, scale and the sums are in fp32, y is
+ * the projection's bf16 output (kc_quantized_matmul), the result is rounded to bf16 once.
+ * kc_adapters_create makes the adapters of one projection: `slots` of them, of ranks up to max_rank (1..128), empty to begin with; in_features a
+ * multiple of 32. kc_adapters_set copies A bf16 [rank, in] and B bf16 [out, rank] into a slot, in place of what it held
+ * (rank 0 empties it; a and b may then be NULL); it returns when the copies are done, behind everything queued before it. */
+typedef struct kc_adapters* kc_adapters_t;
+typedef struct kc_adapter_rows* kc_adapter_rows_t;
+KC_API int kc_adapters_create(kc_ctx_t ctx, int32_t in_features, int32_t out_features, int32_t slots, int32_t max_rank,
+                              kc_adapters_t* out);
+KC_API int kc_adapters_set(kc_adapters_t adapters, int32_t slot, const void* a, const void* b, int32_t rank, float scale,
+                           int32_t on_device);
+KC_API void kc_adapters_free(kc_adapters_t adapters);
+/* Which slot each of a step's m rows uses (HOST i32 [m], -1: none), grouped once for all projections of the step. Any order;
+ * rows of one request best stand together. */
+KC_API int kc_adapter_rows_create(kc_ctx_t ctx, const int32_t* slot_of_row, int32_t m, kc_adapter_rows_t* out);
+KC_API void kc_adapter_rows_free(kc_adapter_rows_t rows);
+/* x bf16 [m, in], 16-byte aligned; y and out bf16 [m, out], the same buffer or apart. A slot that the rows name and
+ * the adapters do not have is refused. Asynchronous on the context's stream; no workspace, so that it may be captured and
+ * several may run at once. */
+KC_API int kc_adapters_apply(kc_adapters_t adapters, kc_adapter_rows_t rows, const void* x_dev, const void* y_dev,
+                             void* out_dev);
+
 /* fast::rms_norm (crates/kiln-mlx/src/fast.rs:36-41): bf16 [rows, dim]. */
 KC_API int kc_rms_norm(kc_ctx_t ctx, const void* x_dev, const void* weight_dev, int32_t rows,
                        int32_t dim, float eps, void* y_dev);

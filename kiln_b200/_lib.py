@@ -101,6 +101,12 @@ _SIGNATURES = {
     "kc_model_set_stream_lane": (C.c_int, [_P, C.c_int32]),
     "kc_quantized_matmul_static": (C.c_int, [_P, _P, _P, C.c_int32, _P]),
     "kc_static_scratch_bytes": (C.c_int64, []),
+    "kc_adapters_create": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "kc_adapters_set": (C.c_int, [_P, C.c_int32, _P, _P, C.c_int32, C.c_float, C.c_int32]),
+    "kc_adapters_free": (None, [_P]),
+    "kc_adapter_rows_create": (C.c_int, [_P, C.POINTER(C.c_int32), C.c_int32, C.POINTER(_P)]),
+    "kc_adapter_rows_free": (None, [_P]),
+    "kc_adapters_apply": (C.c_int, [_P, _P, _P, _P, _P]),
     "kc_rms_norm": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, C.c_float, _P]),
     "kc_paged_attention": (C.c_int, [_P, _P, C.c_int32, _P, C.c_int32, C.c_int32, C.POINTER(KcSeqStep), C.c_int32,
                                      C.c_float, C.c_float, C.c_int32, _P]),

@@ -599,6 +599,80 @@ def verify_accept(ctx: Context, row_tokens: torch.Tensor, row_offsets: torch.Ten
     return committed.view(n, max_commit), ncom, nacc
 
 
+class AdapterRows:
+    """Which adapter each of a step's rows uses (kc_adapter_rows_create): a slot of Adapters, or -1. For all projections of the step."""
+
+    def __init__(self, ctx: Context, slots: Sequence[int]):
+        self.ctx = ctx
+        self._h = C.c_void_p()
+        s = np.ascontiguousarray(slots, dtype=np.int32)
+        if s.ndim != 1:
+            raise ValueError("a slot a row")
+        self.rows = int(s.shape[0])
+        check(L.lib().kc_adapter_rows_create(ctx._h, s.ctypes.data_as(C.POINTER(C.c_int32)), self.rows, C.byref(self._h)))
+        ctx._adopt(self)
+
+    def close(self) -> None:
+        if self._h:
+            L.lib().kc_adapter_rows_free(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Adapters:
+    """The low-rank adapters of one projection (kc_adapters_create): ``slots`` of them, empty until set."""
+
+    def __init__(self, ctx: Context, in_features: int, out_features: int, slots: int, max_rank: int):
+        self.ctx, self.in_features, self.out_features, self.slots, self.max_rank = ctx, in_features, out_features, slots, max_rank
+        self._h = C.c_void_p()
+        check(L.lib().kc_adapters_create(ctx._h, in_features, out_features, slots, max_rank, C.byref(self._h)))
+        ctx._adopt(self)
+
+    def set(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
+        """Copies A bf16 [rank, in] and B bf16 [out, rank], on the host or this device, into the slot."""
+        rank = a.shape[0]
+        if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16 or a.shape != (rank, self.in_features) or b.shape != (self.out_features, rank) or a.is_cuda != b.is_cuda:
+            raise ValueError(f"A bf16 [rank, {self.in_features}] and B bf16 [{self.out_features}, rank] on one device")
+        if a.is_cuda and (a.device.index != self.ctx.device or b.device.index != self.ctx.device):
+            raise ValueError(f"tensors of a context on cuda:{self.ctx.device}")
+        a, b = a.contiguous(), b.contiguous()
+        if a.is_cuda:
+            torch.cuda.current_stream(a.device).synchronize()
+        check(L.lib().kc_adapters_set(self._h, slot, a.data_ptr(), b.data_ptr(), rank, scale, int(a.is_cuda)))
+
+    def clear(self, slot: int) -> None:
+        """Empties the slot: rows that use it keep their y."""
+        check(L.lib().kc_adapters_set(self._h, slot, None, None, 0, 0.0, 0))
+
+    def apply(self, x: torch.Tensor, rows: AdapterRows, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """y + scale B (A x), row by row: x bf16 [m, in], y bf16 [m, out] (a projection's output), ``out`` for the result (y itself: in
+        place). Part of torch's current stream (Context.on_current_stream); the host does not wait."""
+        if out is None:
+            out = torch.empty_like(y)
+        m = rows.rows
+        for name, t, shape in (("x", x, (m, self.in_features)), ("y", y, (m, self.out_features)), ("out", out, (m, self.out_features))):
+            if t.dtype != torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device.type != "cuda" or t.device.index != self.ctx.device:
+                raise ValueError(f"{name}: contiguous bf16 {list(shape)} on cuda:{self.ctx.device}")
+        self.ctx.on_current_stream(L.lib().kc_adapters_apply, self._h, rows._h, x.data_ptr(), y.data_ptr(), out.data_ptr())
+        return out
+
+    def close(self) -> None:
+        if self._h:
+            L.lib().kc_adapters_free(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class QuantizedWeight:
     """One mlx affine-quantised weight re-tiled for the GEMM (ops.rs:362-388 operand)."""
 
@@ -615,8 +689,9 @@ class QuantizedWeight:
                                         self.in_features, bits, group_size, on_dev, C.byref(self._h)))
         ctx._adopt(self)
 
-    def matmul(self, x: torch.Tensor) -> torch.Tensor:
-        """y = x · dequant(W)ᵀ; x bf16 [m, in] on the device."""
+    def matmul(self, x: torch.Tensor, adapters: Optional[Adapters] = None, rows: Optional[AdapterRows] = None) -> torch.Tensor:
+        """y = x · dequant(W)ᵀ; x bf16 [m, in] on the device. With ``adapters`` of this projection, and which one each row uses,
+        what they add to y (Adapters.apply)."""
         assert x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[1] == self.in_features
         m = x.shape[0]
         x = x.contiguous()
@@ -625,6 +700,11 @@ class QuantizedWeight:
         y = torch.empty(m, self.out_features, dtype=torch.bfloat16, device=x.device)
         torch.cuda.current_stream().synchronize()
         check(L.lib().kc_quantized_matmul(self.ctx._h, self._h, x.data_ptr(), m, y.data_ptr()))
+        if adapters is not None:
+            if rows is None or adapters.ctx is not self.ctx or rows.rows != m or (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
+                self.ctx.sync()
+                raise ValueError("adapters of another projection or context, or not a slot for every row")
+            check(L.lib().kc_adapters_apply(adapters._h, rows._h, x.data_ptr(), y.data_ptr(), y.data_ptr()))
         self.ctx.sync()
         return y
 

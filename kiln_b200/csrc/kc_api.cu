@@ -25,6 +25,7 @@
 #include "kc_attn.cuh"
 #include "kc_fused.cuh"
 #include "kc_internal.cuh"
+#include "kc_lora.cuh"
 #include "kc_qlinear.cuh"
 
 using namespace kc;
@@ -697,6 +698,155 @@ extern "C" int kc_quantized_matmul_gemv(kc_ctx_t c, kc_qweight_t q, const void* 
     return fail(KC_ERR_UNSUPPORTED, "kc_quantized_matmul_gemv: a weight of %d x %d does not fit the small-weight lane", q->w.N, q->w.K);
   CK(cudaSetDevice(c->device));
   RC(run_gemv(c, q->w, (const bf16*)x_dev, m, (bf16*)y_dev, q->w.N, q->partial, nullptr));
+  return KC_OK;
+}
+
+// ---------------------------------------------------------------------------
+// adapters
+// ---------------------------------------------------------------------------
+
+struct kc_adapters {
+  kc_ctx* ctx = nullptr;
+  int device = 0, n_in = 0, n_out = 0, slots = 0, max_rank = 0, stride = 0;
+  bf16 *a = nullptr, *b = nullptr;     // [slots][stride][n_in], [slots][n_out][stride]: zero past a slot's rank
+  LoraSlot* meta = nullptr;            // [slots]
+};
+struct kc_adapter_rows {
+  kc_ctx* ctx = nullptr;
+  int device = 0, m = 0, n_tiles = 0, tile_rows = 16, max_slot = -1;
+  LoraTile* tiles = nullptr;           // followed by the rows in their order
+  const int32_t* rows = nullptr;
+};
+
+static void free_adapters(kc_adapters* ad) {
+  cudaFree(ad->a); cudaFree(ad->b); cudaFree(ad->meta);
+  delete ad;
+}
+
+extern "C" int kc_adapters_create(kc_ctx_t c, int32_t in_features, int32_t out_features, int32_t slots, int32_t max_rank, kc_adapters_t* out) {
+  if (!c || !out) return fail(KC_ERR_INVALID, "kc_adapters_create: NULL argument");
+  if (in_features < 32 || in_features % 32 || out_features < 1) return fail(KC_ERR_INVALID, "kc_adapters_create: %d -> %d features (in: a multiple of 32)", in_features, out_features);
+  if (slots < 1 || slots > 1 << 20 || max_rank < 1) return fail(KC_ERR_INVALID, "kc_adapters_create: %d slot(s) of rank %d", slots, max_rank);
+  if (max_rank > LORA_MAX_RANK) return fail(KC_ERR_UNSUPPORTED, "kc_adapters_create: rank %d (at most %d)", max_rank, LORA_MAX_RANK);
+  OnDevice on;
+  CK(on.enter(c->device));
+  kc_adapters* ad = new kc_adapters;
+  ad->ctx = c; ad->device = c->device; ad->n_in = in_features; ad->n_out = out_features; ad->slots = slots; ad->max_rank = max_rank;
+  ad->stride = lora_stride(max_rank);
+  const size_t a_bytes = (size_t)slots * ad->stride * in_features * sizeof(bf16), b_bytes = (size_t)slots * ad->stride * out_features * sizeof(bf16);
+  if (cudaMalloc(&ad->a, a_bytes) != cudaSuccess || cudaMalloc(&ad->b, b_bytes) != cudaSuccess || cudaMalloc(&ad->meta, slots * sizeof(LoraSlot)) != cudaSuccess) {
+    cudaGetLastError();
+    free_adapters(ad);
+    return fail(KC_ERR_OOM, "kc_adapters_create: %zu bytes", a_bytes + b_bytes);
+  }
+  if (cudaMemsetAsync(ad->meta, 0, slots * sizeof(LoraSlot), c->stream) != cudaSuccess) { free_adapters(ad); return fail(KC_ERR_CUDA, "kc_adapters_create: clearing the slots failed"); }
+  g_live++;
+  *out = ad;
+  return KC_OK;
+}
+
+extern "C" void kc_adapters_free(kc_adapters_t ad) {
+  if (!ad) return;
+  OnDevice on;
+  on.enter(ad->device);
+  quiesce(ad->ctx, ad->device);
+  free_adapters(ad);
+  g_live--;
+}
+
+extern "C" int kc_adapters_set(kc_adapters_t ad, int32_t slot, const void* a, const void* b, int32_t rank, float scale, int32_t on_device) {
+  if (!ad || (rank != 0 && (!a || !b))) return fail(KC_ERR_INVALID, "kc_adapters_set: NULL argument");
+  if (slot < 0 || slot >= ad->slots) return fail(KC_ERR_INVALID, "kc_adapters_set: slot %d of %d", slot, ad->slots);
+  if (rank < 0 || rank > ad->max_rank) return fail(KC_ERR_INVALID, "kc_adapters_set: rank %d of at most %d", rank, ad->max_rank);
+  if (!std::isfinite(scale)) return fail(KC_ERR_INVALID, "kc_adapters_set: scale %g", scale);
+  kc_ctx* c = ad->ctx;
+  OnDevice on;
+  CK(on.enter(ad->device));
+  const LoraSlot meta{rank, scale};
+  if (rank > 0) {
+    const size_t a_slot = (size_t)ad->stride * ad->n_in, b_slot = (size_t)ad->stride * ad->n_out;
+    const cudaMemcpyKind kind = on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice;
+    if (rank < ad->stride) {
+      CK(cudaMemsetAsync(ad->a + slot * a_slot, 0, a_slot * sizeof(bf16), c->stream));
+      CK(cudaMemsetAsync(ad->b + slot * b_slot, 0, b_slot * sizeof(bf16), c->stream));
+    }
+    CK(cudaMemcpyAsync(ad->a + slot * a_slot, a, (size_t)rank * ad->n_in * sizeof(bf16), kind, c->stream));
+    CK(cudaMemcpy2DAsync(ad->b + slot * b_slot, ad->stride * sizeof(bf16), b, rank * sizeof(bf16), rank * sizeof(bf16), ad->n_out, kind, c->stream));
+  }
+  CK(cudaMemcpyAsync(ad->meta + slot, &meta, sizeof meta, cudaMemcpyHostToDevice, c->stream));
+  CK(cudaStreamSynchronize(c->stream));
+  return status_verdict(c, "kc_adapters_set");
+}
+
+extern "C" int kc_adapter_rows_create(kc_ctx_t c, const int32_t* slot_of_row, int32_t m, kc_adapter_rows_t* out) {
+  if (!c || !slot_of_row || !out) return fail(KC_ERR_INVALID, "kc_adapter_rows_create: NULL argument");
+  if (m < 1 || m > 1 << 24) return fail(KC_ERR_INVALID, "kc_adapter_rows_create: %d row(s)", m);
+  int max_slot = -1;
+  for (int i = 0; i < m; ++i) {
+    if (slot_of_row[i] < -1) return fail(KC_ERR_INVALID, "kc_adapter_rows_create: row %d uses slot %d", i, slot_of_row[i]);
+    max_slot = std::max(max_slot, slot_of_row[i]);
+  }
+  OnDevice on;
+  CK(on.enter(c->device));
+  std::vector<int32_t> order(m);
+  for (int i = 0; i < m; ++i) order[i] = i;
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return slot_of_row[a] < slot_of_row[b]; });
+  // The largest tiles that still give every SM a CTA and a half: a tile reads its adapter, and eight CTAs take it.
+  std::vector<LoraTile> tiles;
+  int tile_rows = LORA_TILE;
+  for (;; tile_rows /= 2) {
+    tiles.clear();
+    for (int i = 0, j; i < m; i = j) {
+      for (j = i; j < m && slot_of_row[order[j]] == slot_of_row[order[i]]; ++j) {}
+      const int parts = (j - i + tile_rows - 1) / tile_rows;
+      for (int k = 0; k < parts; ++k) {
+        const int first = i + (int)((long long)(j - i) * k / parts), end = i + (int)((long long)(j - i) * (k + 1) / parts);
+        tiles.push_back(LoraTile{slot_of_row[order[i]], first, end - first});
+      }
+    }
+    if (tile_rows == 16 || (long long)tiles.size() * LORA_CTAS * 2 >= 3ll * c->sm_count) break;
+  }
+  kc_adapter_rows* r = new kc_adapter_rows;
+  r->ctx = c; r->device = c->device; r->m = m; r->n_tiles = (int)tiles.size(); r->tile_rows = tile_rows; r->max_slot = max_slot;
+  const size_t t_bytes = tiles.size() * sizeof(LoraTile);
+  cudaError_t e = cudaMalloc(&r->tiles, t_bytes + (size_t)m * 4);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(r->tiles, tiles.data(), t_bytes, cudaMemcpyHostToDevice, c->stream);
+  r->rows = reinterpret_cast<const int32_t*>(reinterpret_cast<uint8_t*>(r->tiles) + t_bytes);
+  if (e == cudaSuccess) e = cudaMemcpyAsync((void*)r->rows, order.data(), (size_t)m * 4, cudaMemcpyHostToDevice, c->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+  if (e != cudaSuccess) {
+    cudaFree(r->tiles);
+    delete r;
+    return fail(e == cudaErrorMemoryAllocation ? KC_ERR_OOM : KC_ERR_CUDA, "kc_adapter_rows_create: %s", cudaGetErrorString(e));
+  }
+  g_live++;
+  *out = r;
+  return KC_OK;
+}
+
+extern "C" void kc_adapter_rows_free(kc_adapter_rows_t r) {
+  if (!r) return;
+  OnDevice on;
+  on.enter(r->device);
+  quiesce(r->ctx, r->device);
+  cudaFree(r->tiles);
+  delete r;
+  g_live--;
+}
+
+extern "C" int kc_adapters_apply(kc_adapters_t ad, kc_adapter_rows_t r, const void* x_dev, const void* y_dev, void* out_dev) {
+  if (!ad || !r || !x_dev || !y_dev || !out_dev) return fail(KC_ERR_INVALID, "kc_adapters_apply: NULL argument");
+  if (ad->ctx != r->ctx) return fail(KC_ERR_INVALID, "kc_adapters_apply: adapters and rows belong to different contexts");
+  if (r->max_slot >= ad->slots) return fail(KC_ERR_INVALID, "kc_adapters_apply: rows use slot %d of %d", r->max_slot, ad->slots);
+  if ((uintptr_t)x_dev % 16 || (uintptr_t)y_dev % 2 || (uintptr_t)out_dev % 2) return fail(KC_ERR_INVALID, "kc_adapters_apply: x must be 16-byte aligned, y and out 2-byte");
+  kc_ctx* c = ad->ctx;
+  OnDevice on;
+  CK(on.enter(ad->device));
+  LoraParams p{};
+  p.x = (const bf16*)x_dev; p.y = (const bf16*)y_dev; p.out = (bf16*)out_dev;
+  p.a = ad->a; p.b = ad->b; p.slots = ad->meta; p.tiles = r->tiles; p.rows = r->rows;
+  p.n_tiles = r->n_tiles; p.tile_rows = r->tile_rows; p.n_in = ad->n_in; p.n_out = ad->n_out; p.stride = ad->stride;
+  LAUNCH(c, KC_PROF_GEMM, 1, lora_apply(p, c->stream));
   return KC_OK;
 }
 
