@@ -199,6 +199,18 @@ def _alias_bf16(ptr: int, shape, device: int) -> torch.Tensor:
     return t.view(torch.bfloat16)
 
 
+# torch.cuda.current_stream(device).cuda_stream without the stream object that takes a microsecond to make
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _expect(ctx: "Context", name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
+    """A contiguous tensor of that type and shape on the context's device, or ValueError (cheap tests: this runs per call of
+    an operator that takes a few microseconds)."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda or t.get_device() != ctx.device:
+        raise ValueError(f"{name}: contiguous {dtype} {list(shape)} on cuda:{ctx.device}")
+
+
 def _ptr(t) -> int:
     if isinstance(t, torch.Tensor):
         return t.data_ptr()
@@ -247,7 +259,7 @@ class Context:
         context's device: behind what that stream and the context's hold, and ahead of what either is given later. The host
         waits for nothing, also in a capture into a graph. A program that makes the context's stream torch's current one
         (``torch.cuda.ExternalStream(ctx.stream)``) spares the two events that this takes."""
-        current = torch.cuda.current_stream(self.device).cuda_stream
+        current = _raw_stream(self.device)
         if current == self._stream:
             check(call(*args))
             return
@@ -564,21 +576,21 @@ def sample_rows(ctx: Context, logits: torch.Tensor, params, uniforms: torch.Tens
     were kept: (int32 [rows], float32 [rows]); see kc_sample_rows. ``params``: pack_sampling's tensor or a sequence of
     SamplingParams; ``uniforms``: float32 [rows] in [0, 1) on the device. ``out`` and ``logprobs``: where the results go.
     Part of torch's current stream (Context.on_current_stream); the host does not wait."""
-    if logits.dtype != torch.bfloat16 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    if logits.dtype is not torch.bfloat16 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits: bf16 [rows, vocab], the values of a row side by side")
     rows, vocab = logits.shape
     if not isinstance(params, torch.Tensor):
         params = pack_sampling(params, logits.device)
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        out = logits.new_empty(rows, dtype=torch.int32)
     if logprobs is None:
-        logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    for name, t, dtype, shape in (("params", params, torch.int32, (rows, 4)), ("uniforms", uniforms, torch.float32, (rows,)),
-                                  ("out", out, torch.int32, (rows,)), ("logprobs", logprobs, torch.float32, (rows,))):
-        if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous {dtype} {list(shape)}")
-    if any(t.device.type != "cuda" or t.device.index != ctx.device for t in (logits, params, uniforms, out, logprobs)):
-        raise ValueError(f"tensors of a context on cuda:{ctx.device}")
+        logprobs = logits.new_empty(rows, dtype=torch.float32)
+    _expect(ctx, "params", params, torch.int32, (rows, 4))
+    _expect(ctx, "uniforms", uniforms, torch.float32, (rows,))
+    _expect(ctx, "out", out, torch.int32, (rows,))
+    _expect(ctx, "logprobs", logprobs, torch.float32, (rows,))
+    if logits.get_device() != ctx.device:
+        raise ValueError(f"logits: on cuda:{ctx.device}")
     ctx.on_current_stream(L.lib().kc_sample_rows, ctx._h, logits.data_ptr(), logits.stride(0), rows, vocab, params.data_ptr(), uniforms.data_ptr(),
                           out.data_ptr(), logprobs.data_ptr())
     return out, logprobs
@@ -655,9 +667,9 @@ class Adapters:
         if out is None:
             out = torch.empty_like(y)
         m = rows.rows
-        for name, t, shape in (("x", x, (m, self.in_features)), ("y", y, (m, self.out_features)), ("out", out, (m, self.out_features))):
-            if t.dtype != torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device.type != "cuda" or t.device.index != self.ctx.device:
-                raise ValueError(f"{name}: contiguous bf16 {list(shape)} on cuda:{self.ctx.device}")
+        _expect(self.ctx, "x", x, torch.bfloat16, (m, self.in_features))
+        _expect(self.ctx, "y", y, torch.bfloat16, (m, self.out_features))
+        _expect(self.ctx, "out", out, torch.bfloat16, (m, self.out_features))
         self.ctx.on_current_stream(L.lib().kc_adapters_apply, self._h, rows._h, x.data_ptr(), y.data_ptr(), out.data_ptr())
         return out
 
@@ -787,10 +799,9 @@ class AttentionPlan:
             raise ValueError("the plan or its pools are closed")
         dim = self.kv.spec.head_dim
         if out is None:
-            out = torch.empty(self.tokens, self.heads * dim, dtype=torch.bfloat16, device=q.device)
-        for name, t, shape in (("q", q, (self.tokens, self.heads, dim)), ("out", out, (self.tokens, self.heads * dim))):
-            if t.dtype != torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device.type != "cuda" or t.device.index != self.ctx.device:
-                raise ValueError(f"{name}: contiguous bf16 {list(shape)} on cuda:{self.ctx.device}")
+            out = q.new_empty(self.tokens, self.heads * dim, dtype=torch.bfloat16)
+        _expect(self.ctx, "q", q, torch.bfloat16, (self.tokens, self.heads, dim))
+        _expect(self.ctx, "out", out, torch.bfloat16, (self.tokens, self.heads * dim))
         self.ctx.on_current_stream(L.lib().kc_attn_plan_run, self._h, layer, q.data_ptr(), scale, softcap, window, out.data_ptr())
         return out
 
