@@ -713,7 +713,7 @@ struct kc_adapters {
 };
 struct kc_adapter_rows {
   kc_ctx* ctx = nullptr;
-  int device = 0, m = 0, n_tiles = 0, tile_rows = 16, max_slot = -1;
+  int device = 0, m = 0, n_tiles = 0, max_slot = -1;
   LoraTile* tiles = nullptr;           // followed by the rows in their order
   const int32_t* rows = nullptr;
 };
@@ -791,23 +791,13 @@ extern "C" int kc_adapter_rows_create(kc_ctx_t c, const int32_t* slot_of_row, in
   std::vector<int32_t> order(m);
   for (int i = 0; i < m; ++i) order[i] = i;
   std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return slot_of_row[a] < slot_of_row[b]; });
-  // The largest tiles that still give every SM a CTA and a half: a tile reads its adapter, and eight CTAs take it.
   std::vector<LoraTile> tiles;
-  int tile_rows = LORA_TILE;
-  for (;; tile_rows /= 2) {
-    tiles.clear();
-    for (int i = 0, j; i < m; i = j) {
-      for (j = i; j < m && slot_of_row[order[j]] == slot_of_row[order[i]]; ++j) {}
-      const int parts = (j - i + tile_rows - 1) / tile_rows;
-      for (int k = 0; k < parts; ++k) {
-        const int first = i + (int)((long long)(j - i) * k / parts), end = i + (int)((long long)(j - i) * (k + 1) / parts);
-        tiles.push_back(LoraTile{slot_of_row[order[i]], first, end - first});
-      }
-    }
-    if (tile_rows == 16 || (long long)tiles.size() * LORA_CTAS * 2 >= 3ll * c->sm_count) break;
+  for (int i = 0, j; i < m; i = j) {
+    for (j = i; j < m && slot_of_row[order[j]] == slot_of_row[order[i]]; ++j) {}
+    for (int k = i; k < j; k += LORA_TILE) tiles.push_back(LoraTile{slot_of_row[order[i]], k, std::min(LORA_TILE, j - k)});
   }
   kc_adapter_rows* r = new kc_adapter_rows;
-  r->ctx = c; r->device = c->device; r->m = m; r->n_tiles = (int)tiles.size(); r->tile_rows = tile_rows; r->max_slot = max_slot;
+  r->ctx = c; r->device = c->device; r->m = m; r->n_tiles = (int)tiles.size(); r->max_slot = max_slot;
   const size_t t_bytes = tiles.size() * sizeof(LoraTile);
   cudaError_t e = cudaMalloc(&r->tiles, t_bytes + (size_t)m * 4);
   if (e == cudaSuccess) e = cudaMemcpyAsync(r->tiles, tiles.data(), t_bytes, cudaMemcpyHostToDevice, c->stream);
@@ -845,8 +835,8 @@ extern "C" int kc_adapters_apply(kc_adapters_t ad, kc_adapter_rows_t r, const vo
   LoraParams p{};
   p.x = (const bf16*)x_dev; p.y = (const bf16*)y_dev; p.out = (bf16*)out_dev;
   p.a = ad->a; p.b = ad->b; p.slots = ad->meta; p.tiles = r->tiles; p.rows = r->rows;
-  p.n_tiles = r->n_tiles; p.tile_rows = r->tile_rows; p.n_in = ad->n_in; p.n_out = ad->n_out; p.stride = ad->stride;
-  LAUNCH(c, KC_PROF_GEMM, 1, lora_apply(p, c->stream));
+  p.n_tiles = r->n_tiles; p.n_in = ad->n_in; p.n_out = ad->n_out; p.stride = ad->stride;
+  LAUNCH(c, KC_PROF_GEMM, 1, lora_apply(p, c->sm_count, c->stream));
   return KC_OK;
 }
 

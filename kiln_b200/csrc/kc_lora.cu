@@ -1,22 +1,26 @@
 // What low-rank adapters add to a projection's rows: out_i = y_i + s_a B_a (A_a x_i), a the adapter of row i.
 //
-// One launch. Rows are grouped by adapter on the host (kc_adapter_rows_create) into tiles of at most 64, and a tile is a cluster's
-// of eight CTAs: each multiplies an eighth of the features of x with an eighth of A's columns, the partial t = A x [rows, rank] meet in
-// the cluster's shared memory, and each CTA takes an eighth of the projection's features through B and adds them to y.
-// So t never goes through memory, x, y and the adapter are read once a tile, and no workspace or order of atomics is involved.
+// One launch. Rows are grouped by adapter on the host (kc_adapter_rows_create) into tiles of at most 16, and a tile is a cluster's
+// of eight, four or two CTAs: each multiplies its share of the features of x with A's columns, the partial t = A x [rows, rank] meet
+// in the cluster's shared memory, and each CTA takes its share of the projection's features through B and adds them to y. So t
+// never goes through memory, and no workspace or order of atomics is involved.
 //
-// Both products are mma.sync m16n8k16: what bounds the operator is memory, rank / 2 operations a byte of y, far below what either
-// kind of tensor instruction does, and these take their operands from registers as they come from memory. The contraction's order is free,
-// so a lane's elements of an operand are neighbours: 16-byte loads of x and A, and of B where ranks are stored by 32; the
-// columns of B are dealt so that a lane has eight neighbouring features of y.
+// Both products are mma.sync m16n8k16, which takes its operands from registers as they come from memory. The contraction's order is
+// free, so a lane's elements of an operand are neighbours: 16-byte loads of x and A, 8 to 32 bytes of B; and the columns of B
+// are dealt so that a lane has eight neighbouring features of y.
 //
-// t is summed in fp32, multiplied by s and goes into the second product as two bf16 numbers (its rounded value and what that leaves:
-// 2^-17 of it is lost, a 256th of the output's own step); y is added in fp32 and the result rounded once.
+// t is summed in fp32, multiplied by s and rounded to bf16 for the second product, as a model's activations are between two
+// projections: with what that leaves as a second bf16 number the result was 0.1 of its own rounding nearer, for twice the instructions
+// of the product (2048 rows of rank 64: 118 -> 94 us without). y is added in fp32 and the result rounded once.
+//
+// What bounds it. Few rows: launch, two latencies of memory and two exchanges, 4.8 us; 32 rows of an adapter each into 28672 features
+// read 29 MB of B in 13.4 us, of which 5.7 are memory's. Many rows: the 16 rows of a tile share what they read of B, so that
+// L1 sees four times y; 2048 rows of rank 64 into 28672 features take 89 us, 44 at a copy's rate. Tiles of 32 and 64 rows with B through
+// shared memory were built and are no faster (94 and 155 us at these sizes): a CTA's fixed part, a barrier a round and fewer clusters at once
+// cost what they save.
 #include "kc_lora.cuh"
 
 #include "kc_umma.cuh"
-
-#include <algorithm>
 
 namespace kc {
 
@@ -33,36 +37,62 @@ __device__ __forceinline__ float peer_float(const float* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(smem_u32(p), rank)) : "memory");
   return v;
 }
-
-// Shared memory of a CTA: partial sums of its warps [8][16][pad], its t [16 MT][stride], t in two parts [2][16 MT][stride + 8].
-__host__ __device__ constexpr int lora_pad(int stride) { return stride + 8; }
-constexpr size_t lora_smem(int stride, int mt) {
-  return (size_t)LORA_WARPS * 16 * lora_pad(stride) * 4 + (size_t)16 * mt * stride * 4 + (size_t)2 * 16 * mt * lora_pad(stride) * 2;
+__device__ __forceinline__ void peer_put(bf16* p, uint32_t rank, bf16 v) {
+  asm volatile("st.shared::cluster.b16 [%0], %1;" ::"r"(cluster_addr(smem_u32(p), rank)), "h"(__bfloat16_as_ushort(v)) : "memory");
 }
 
-// MT: row blocks of 16 in a tile; the CTA's eight warps are MT of them times 8 / MT parts of its features. VEC: rows of y and out
-// start on 16-byte boundaries.
-template <int MT, bool VEC>
-__global__ void __launch_bounds__(LORA_THREADS, 2)
+// N registers (2, 4 or 8) from memory on a boundary of their size.
+template <int N>
+__device__ __forceinline__ void load_regs(uint32_t* r, const void* from) {
+  if constexpr (N == 8) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(from) : "memory");
+  } else if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(from);
+    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(from);
+    r[0] = v.x; r[1] = v.y;
+  }
+}
+
+// A kernel's shape: CTAs of a cluster, and R, the ranks as they are stored.
+template <int CTAS_, int R_>
+struct LoraShape {
+  static constexpr int CTAS = CTAS_, R = R_, ROWS = LORA_TILE;
+  static constexpr int PARTS = 8 / CTAS;           // eighths of the features of x that a CTA has
+  static constexpr int RS = R < 64 ? R : 64;       // ranks of a step of the first product
+  static constexpr int PAD = R + 8;                // of a row of t: 16-byte pieces of neighbouring rows lie in different banks
+  static constexpr int PART = RS + 4;
+  static constexpr int W = R / 8;                  // registers of a lane's quarter of the ranks
+  // Rounds (32 features a warp) that a warp has B and y of, and as many on their way; CTAs of an SM: what 65536 registers hold.
+  static constexpr int U = R <= 32 ? 2 : 1;
+  static constexpr int RESIDENT = R <= 64 ? 2 : 1;
+  // Shared memory of a CTA: partial sums of its warps for a step [8][ROWS][PART], its parts' t [PARTS][ROWS][R], the cluster's t [ROWS][PAD].
+  static constexpr size_t SMEM = ((size_t)LORA_WARPS * ROWS * PART + (size_t)PARTS * ROWS * R) * 4 + (size_t)ROWS * PAD * 2;
+  static_assert(SMEM <= 227 * 1024 / RESIDENT - 1024, "shared memory");
+};
+
+// VEC: rows of y and out start on 16-byte boundaries.
+template <typename S, bool VEC>
+__global__ void __launch_bounds__(LORA_THREADS, S::RESIDENT)
 lora_kernel(const LoraParams p) {
-  constexpr int KP = LORA_WARPS / MT;
-  extern __shared__ __align__(16) uint8_t lora_smem_base[];
-  const int R = p.stride, pad = lora_pad(R);
-  float* part = reinterpret_cast<float*>(lora_smem_base);
-  float* sum = part + LORA_WARPS * 16 * pad;
-  bf16* th = reinterpret_cast<bf16*>(sum + 16 * MT * R);
-  bf16* tl = th + 16 * MT * pad;
-  __shared__ int rows[16 * MT];
+  constexpr int R = S::R, RS = S::RS, NB = RS / 8, PAD = S::PAD, PART = S::PART, W = S::W, U = S::U, ROWS = S::ROWS, CTAS = S::CTAS, PARTS = S::PARTS;
+  extern __shared__ __align__(16) uint8_t lora_smem[];
+  float* part = reinterpret_cast<float*>(lora_smem);
+  float* sum = part + LORA_WARPS * ROWS * PART;
+  bf16* ts = reinterpret_cast<bf16*>(sum + PARTS * ROWS * R);
+  __shared__ int rows[ROWS];
   pdl_launch_dependents();
   cluster_arrive();                    // waited for before the first access to another CTA's shared memory: it has started by then
-  const int rank = blockIdx.x % LORA_CTAS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rank = blockIdx.x % CTAS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_wait();
-  const LoraTile tile = p.tiles[blockIdx.x / LORA_CTAS];
+  const LoraTile tile = p.tiles[blockIdx.x / CTAS];
   const LoraSlot slot = tile.slot >= 0 ? p.slots[tile.slot] : LoraSlot{0, 0.f};
-  if (threadIdx.x < 16 * MT) rows[threadIdx.x] = p.rows[tile.first + min((int)threadIdx.x, tile.n - 1)];
+  if (threadIdx.x < ROWS) rows[threadIdx.x] = p.rows[tile.first + min((int)threadIdx.x, tile.n - 1)];
   __syncthreads();
   cluster_wait();
-  const int blocks = (p.n_out + 31) / 32, b0 = (int)((long long)blocks * rank / LORA_CTAS), b1 = (int)((long long)blocks * (rank + 1) / LORA_CTAS);
+  const int blocks = (p.n_out + 31) / 32, b0 = (int)((long long)blocks * rank / CTAS), b1 = (int)((long long)blocks * (rank + 1) / CTAS);
 
   if (slot.rank == 0) {                // no adapter: the rows as they are
     if (p.out != p.y) {
@@ -75,166 +105,189 @@ lora_kernel(const LoraParams p) {
     }
     return;                            // all CTAs of the cluster
   }
-  // ranks in use, in whole steps
-  const int steps = R == 16 ? 1 : (slot.rank + 31) / 32 * 2;   // of 16
 
-  // ---- t = A x over this CTA's features: warp = (row block, part) ----
+  // ---- what a warp needs of B and y for 32 features. Column 2 t' + e of column block j is feature 8 t' + 2 j + e, so that a lane's
+  // columns are eight neighbours; its ranks are a quarter of them, the t-th ----
+  const size_t y_at[2] = {(size_t)rows[g] * p.n_out + t * 8, (size_t)rows[g + 8] * p.n_out + t * 8};
+  const bf16* bank = p.b + (size_t)tile.slot * p.n_out * R + t * (R / 4);
+  struct Block { uint32_t w[4][W], y[2][4]; };
+  auto load = [&](Block& b, int blk) {
+    if (blk >= b1) return;
+    if constexpr (VEC) {
+      if (blk * 32 + t * 8 < p.n_out) {
+        if (g < tile.n) load_regs<4>(b.y[0], p.y + y_at[0] + blk * 32);
+        if (g + 8 < tile.n) load_regs<4>(b.y[1], p.y + y_at[1] + blk * 32);
+      }
+    }
+    const int feature = blk * 32 + (g >> 1) * 8 + (g & 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bf16* from = bank + (size_t)min(feature + 2 * j, p.n_out - 1) * R;
+      if constexpr (W == 16) { load_regs<8>(b.w[j], from); load_regs<8>(b.w[j] + 8, from + 16); }
+      else load_regs<W>(b.w[j], from);
+    }
+  };
+  Block cur[U];
+  auto load_first = [&]() {
+#pragma unroll
+    for (int i = 0; i < U; ++i) load(cur[i], b0 + warp + i * LORA_WARPS);
+  };
+  constexpr bool EARLY = R == 16;      // under the first product already, where the registers are there
+  if (EARLY) load_first();
+
+  // ---- t = A x over this CTA's parts of the features, an eighth of a part a warp. The parts are the same for every size of cluster,
+  // so that a row's bits do not hang on it ----
   {
-    const int mt = warp % MT, kp = warp / MT;
-    const int chunks = p.n_in / 32, parts = LORA_CTAS * KP, me = rank * KP + kp;
-    const int c0 = (int)((long long)chunks * me / parts), c1 = (int)((long long)chunks * (me + 1) / parts);
-    const bf16* x0 = p.x + (size_t)rows[mt * 16 + g] * p.n_in + t * 8;
-    const bf16* x1 = p.x + (size_t)rows[mt * 16 + g + 8] * p.n_in + t * 8;
-    const bf16* a = p.a + ((size_t)tile.slot * R + g) * p.n_in + t * 8;
-    // Ranks 32 at a time: four column blocks of eight, or the two there are.
-    for (int s = 0; s < steps; s += 2) {
-      float acc[4][4] = {};
-      if (mt * 16 < tile.n) {
-#pragma unroll 4
+    const int chunks = p.n_in / 32, used = (slot.rank + RS - 1) / RS;   // steps of ranks in use
+    const bf16 *x0 = p.x + (size_t)rows[g] * p.n_in + t * 8, *x1 = p.x + (size_t)rows[g + 8] * p.n_in + t * 8;
+    for (int i = 0; i < PARTS; ++i) {
+      const int me = (rank * PARTS + i) * LORA_WARPS + warp;
+      const int c0 = (int)((long long)chunks * me / (8 * LORA_WARPS)), c1 = (int)((long long)chunks * (me + 1) / (8 * LORA_WARPS));
+      for (int s = 0; s < used; ++s) {
+        const bf16* a = p.a + ((size_t)tile.slot * R + s * RS + g) * p.n_in + t * 8;
+        float acc[NB][4] = {};
+#pragma unroll 2
         for (int c = c0; c < c1; ++c) {
+          uint4 w[NB];
+#pragma unroll
+          for (int j = 0; j < NB; ++j) w[j] = *reinterpret_cast<const uint4*>(a + (size_t)j * 8 * p.n_in + (size_t)c * 32);
           const uint4 u0 = *reinterpret_cast<const uint4*>(x0 + (size_t)c * 32), u1 = *reinterpret_cast<const uint4*>(x1 + (size_t)c * 32);
-          uint4 w[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < 2 || steps > 1) w[j] = *reinterpret_cast<const uint4*>(a + (size_t)(s * 16 + j * 8) * p.n_in + (size_t)c * 32);
+          for (int j = 0; j < NB; ++j) {
+            mma_bf16(acc[j], u0.x, u1.x, u0.y, u1.y, w[j].x, w[j].y);
+            mma_bf16(acc[j], u0.z, u1.z, u0.w, u1.w, w[j].z, w[j].w);
+          }
+        }
+        if (i + s > 0) __syncthreads();   // the last partial sums have been read
+        float* to = part + (warp * ROWS + g) * PART + t * 2;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < 2 || steps > 1) {
-              mma_bf16(acc[j], u0.x, u1.x, u0.y, u1.y, w[j].x, w[j].y);
-              mma_bf16(acc[j], u0.z, u1.z, u0.w, u1.w, w[j].z, w[j].w);
-            }
+        for (int j = 0; j < NB; ++j) {
+          *reinterpret_cast<float2*>(to + j * 8) = make_float2(acc[j][0], acc[j][1]);
+          *reinterpret_cast<float2*>(to + 8 * PART + j * 8) = make_float2(acc[j][2], acc[j][3]);
+        }
+        __syncthreads();
+        for (int k = threadIdx.x; k < tile.n * RS; k += LORA_THREADS) {
+          const int row = k / RS, r = k % RS;
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < LORA_WARPS; ++w) v += part[(w * ROWS + row) * PART + r];
+          sum[(i * ROWS + row) * R + s * RS + r] = v;
         }
       }
-      float* to = part + (warp * 16 + g) * pad + s * 16 + t * 2;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < 2 || steps > 1) {
-          *reinterpret_cast<float2*>(to + j * 8) = make_float2(acc[j][0], acc[j][1]);
-          *reinterpret_cast<float2*>(to + 8 * pad + j * 8) = make_float2(acc[j][2], acc[j][3]);
-        }
     }
-  }
-  __syncthreads();
-  const int live = min(MT, (tile.n + 15) / 16), used = steps * 16, items = live * 16 * used;
-  for (int i = threadIdx.x; i < items; i += LORA_THREADS) {
-    const int row = i / used, r = i - row * used, mt = row >> 4;
-    float v = 0.f;
-#pragma unroll
-    for (int kp = 0; kp < KP; ++kp) v += part[((kp * MT + mt) * 16 + (row & 15)) * pad + r];
-    sum[row * R + r] = v;
   }
   cluster_sync();
-  // ---- the cluster's t, in the order of its CTAs; ranks past the adapter's own have no part, whatever x holds ----
-  for (int i = threadIdx.x; i < items; i += LORA_THREADS) {
-    const int row = i / used, r = i - row * used;
-    float v = 0.f;
+  if (!EARLY) load_first();            // they arrive under the exchange
+  // ---- the cluster's t, in the order of its parts, rounded to bf16; ranks past the adapter's own are zero, whatever x holds. Of
+  // many values each CTA adds up its share and hands it to all, of few every CTA all of them ----
+  {
+    const int items = tile.n * R;
+    const bool shared = items > 1024;
+    const int from = shared ? items * rank / CTAS : 0, to = shared ? items * (rank + 1) / CTAS : items;
+    for (int i = from + threadIdx.x; i < to; i += LORA_THREADS) {
+      const int row = i / R, r = i % R;
+      float v = 0.f;
+      if (r < slot.rank) {
+        float q[8];
 #pragma unroll
-    for (int k = 0; k < LORA_CTAS; ++k) v += peer_float(&sum[row * R + r], k);
-    v = r < slot.rank ? v * slot.scale : 0.f;
-    const bf16 hi = __float2bfloat16_rn(v);
-    const float rest = v - __bfloat162float(hi);
-    th[row * pad + r] = hi;
-    tl[row * pad + r] = __float2bfloat16_rn(rest == rest ? rest : 0.f);   // of an infinite value nothing is left
-  }
-  cluster_arrive();                    // no CTA leaves while another one reads its sums; the barrier also joins this CTA's warps
-  cluster_wait();
-
-  // ---- out = y + B t: a warp has 32 features at a time. Column 2 t' + e of column block j is feature 8 t' + 2 j + e, so that a
-  // lane's columns are eight neighbours ----
-  const bf16* bank = p.b + (size_t)tile.slot * p.n_out * R;
-  for (int blk = b0 + warp; blk < b1; blk += LORA_WARPS) {
-    const int f0 = blk * 32, mine = f0 + t * 8;
-    float acc[MT][4][4] = {};
-    uint4 y[MT][2];
-    if (VEC) {
+        for (int k = 0; k < 8; ++k) q[k] = peer_float(&sum[(k % PARTS * ROWS + row) * R + r], k / PARTS);
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (m * 16 + h * 8 + g < tile.n && mine < p.n_out) y[m][h] = *reinterpret_cast<const uint4*>(p.y + (size_t)rows[m * 16 + h * 8 + g] * p.n_out + mine);
-    }
-    const int feature = f0 + (g >> 1) * 8 + (g & 1);
-    if (R == 16) {
-      uint2 w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint2*>(bank + (size_t)min(feature + 2 * j, p.n_out - 1) * 16 + t * 4);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m >= live) break;
-#pragma unroll
-        for (int part2 = 0; part2 < 2; ++part2) {
-          const bf16* src = (part2 ? tl : th) + (m * 16 + g) * pad + t * 4;
-          const uint2 v0 = *reinterpret_cast<const uint2*>(src), v1 = *reinterpret_cast<const uint2*>(src + 8 * pad);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mma_bf16(acc[m][j], v0.x, v1.x, v0.y, v1.y, w[j].x, w[j].y);
-        }
+        for (int k = 0; k < 8; ++k) v += q[k];
+        v *= slot.scale;
       }
-    } else {
+      const bf16 b = __float2bfloat16_rn(v);
+      if (!shared) { ts[row * PAD + r] = b; continue; }
+#pragma unroll
+      for (int k = 0; k < CTAS; ++k) peer_put(&ts[row * PAD + r], k, b);
+    }
+  }
+  cluster_sync();                      // also: no CTA leaves while another one reads its sums
+
+  // ---- out = y + B t: t stays in registers ----
+  uint32_t v[2][W];                    // [row][ranks]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const bf16* from = ts + (h * 8 + g) * PAD + t * (R / 4);
+#pragma unroll
+    for (int k = 0; k < W; k += 2) {
+      const uint2 q = *reinterpret_cast<const uint2*>(from + 2 * k);
+      v[h][k] = q.x; v[h][k + 1] = q.y;
+    }
+  }
 #pragma unroll 1
-      for (int s = 0; s < steps; s += 2) {
-        uint4 w[4];
+  for (int blk = b0 + warp; blk < b1; blk += LORA_WARPS * U) {
+    Block next[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(bank + (size_t)min(feature + 2 * j, p.n_out - 1) * R + s * 16 + t * 8);
+    for (int i = 0; i < U; ++i) load(next[i], blk + (U + i) * LORA_WARPS);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if (m >= live) break;
+    for (int i = 0; i < U; ++i) {
+      const int at = blk + i * LORA_WARPS, mine = at * 32 + t * 8;
+      if (at < b1) {
+        float acc[4][4] = {};
 #pragma unroll
-          for (int part2 = 0; part2 < 2; ++part2) {
-            const bf16* src = (part2 ? tl : th) + (m * 16 + g) * pad + s * 16 + t * 8;
-            const uint4 v0 = *reinterpret_cast<const uint4*>(src), v1 = *reinterpret_cast<const uint4*>(src + 8 * pad);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < W; k += 2) mma_bf16(acc[j], v[0][k], v[1][k], v[0][k + 1], v[1][k + 1], cur[i].w[j][k], cur[i].w[j][k + 1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h * 8 + g >= tile.n || mine >= p.n_out) continue;
+          bf16* to = p.out + y_at[h] + (size_t)at * 32;
+          if constexpr (VEC) {
+            uint32_t o[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              mma_bf16(acc[m][j], v0.x, v1.x, v0.y, v1.y, w[j].x, w[j].y);
-              mma_bf16(acc[m][j], v0.z, v1.z, v0.w, v1.w, w[j].z, w[j].w);
+              const float2 f = unpack_bf162(cur[i].y[h][j]);
+              o[j] = pack_bf162(f.x + acc[j][2 * h], f.y + acc[j][2 * h + 1]);
             }
+            *reinterpret_cast<uint4*>(to) = make_uint4(o[0], o[1], o[2], o[3]);
+          } else {
+            const bf16* from = p.y + y_at[h] + (size_t)at * 32;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (mine + e < p.n_out) to[e] = __float2bfloat16_rn(__bfloat162float(from[e]) + acc[e >> 1][2 * h + (e & 1)]);
           }
         }
       }
+      cur[i] = next[i];
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = m * 16 + h * 8 + g;
-        if (r >= tile.n || mine >= p.n_out) continue;
-        const size_t at = (size_t)rows[r] * p.n_out + mine;
-        if (VEC) {
-          const uint32_t v[4] = {y[m][h].x, y[m][h].y, y[m][h].z, y[m][h].w};
-          uint32_t o[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack_bf162(v[j]);
-            o[j] = pack_bf162(f.x + acc[m][j][2 * h], f.y + acc[m][j][2 * h + 1]);
-          }
-          *reinterpret_cast<uint4*>(p.out + at) = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (mine + e < p.n_out) p.out[at + e] = __float2bfloat16_rn(__bfloat162float(p.y[at + e]) + acc[m][e >> 1][2 * h + (e & 1)]);
-        }
-      }
   }
 }
 
-template <int MT, bool VEC>
-cudaError_t launch_as(const LoraParams& p, cudaStream_t s) {
-  static DeviceOnce configured;   // the attribute belongs to the device's copy of the kernel
-  if (configured.first_on_current_device()) {
-    cudaError_t e = cudaFuncSetAttribute(lora_kernel<MT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lora_smem(LORA_MAX_RANK, MT));
-    if (e != cudaSuccess) { configured.forget_current_device(); return e; }
-  }
-  return launch_k_cluster(LORA_CTAS, lora_kernel<MT, VEC>, dim3(p.n_tiles * LORA_CTAS), dim3(LORA_THREADS), lora_smem(p.stride, MT), s, p);
+template <typename S>
+cudaError_t launch(const LoraParams& p, cudaStream_t s) {
+  const bool vec = p.n_out % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  auto as = [&](auto kernel, DeviceOnce& configured) {   // the attribute belongs to the device's copy of the kernel
+    if (configured.first_on_current_device()) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+      if (e != cudaSuccess) { configured.forget_current_device(); return e; }
+    }
+    return launch_k_cluster(S::CTAS, kernel, dim3(p.n_tiles * S::CTAS), dim3(LORA_THREADS), S::SMEM, s, p);
+  };
+  static DeviceOnce with_vec, without;
+  return vec ? as(lora_kernel<S, true>, with_vec) : as(lora_kernel<S, false>, without);
+}
+
+// The largest clusters of which the SMs hold all at once (a cluster lies in one group of SMs: of 296 places for CTAs clusters of eight
+// take 256, of four 284), else two CTAs a tile, whose fixed part weighs least. Rank 16, 4096 -> 28672 features, with 8, 4 and 2 CTAs,
+// us: 32 tiles 19.3, 24.7, 39.8; 34 28.3, 26.2, 40.0; 70 45.6, 33.4, 44.8; 74 46.9, 50.4, 45.6; 4096 -> 4096: 7.0, 7.6, 10.7; 10.3, 8.5,
+// 10.8; 18.2, 11.0, 14.4; 19.0, 16.4, 14.3.
+template <int R>
+cudaError_t launch_rank(const LoraParams& p, int sm_count, cudaStream_t s) {
+  const long long places = (long long)sm_count * LoraShape<8, R>::RESIDENT;
+  if (p.n_tiles * 8 <= places * 87 / 100) return launch<LoraShape<8, R>>(p, s);
+  if (p.n_tiles * 4 <= places * 96 / 100) return launch<LoraShape<4, R>>(p, s);
+  return launch<LoraShape<2, R>>(p, s);
 }
 
 }  // namespace
 
-cudaError_t lora_apply(const LoraParams& p, cudaStream_t s) {
-  if (p.n_tiles < 1 || p.n_in % 32 || p.stride > LORA_MAX_RANK) return cudaErrorInvalidValue;
-  const bool vec = p.n_out % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-  switch (p.tile_rows) {
-    case 16: return vec ? launch_as<1, true>(p, s) : launch_as<1, false>(p, s);
-    case 32: return vec ? launch_as<2, true>(p, s) : launch_as<2, false>(p, s);
-    case 64: return vec ? launch_as<4, true>(p, s) : launch_as<4, false>(p, s);
+cudaError_t lora_apply(const LoraParams& p, int sm_count, cudaStream_t s) {
+  if (p.n_tiles < 1 || p.n_in % 32) return cudaErrorInvalidValue;
+  switch (p.stride) {
+    case 16: return launch_rank<16>(p, sm_count, s);
+    case 32: return launch_rank<32>(p, sm_count, s);
+    case 64: return launch_rank<64>(p, sm_count, s);
+    case 128: return launch_rank<128>(p, sm_count, s);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -5,8 +5,7 @@
 
 namespace kc {
 
-constexpr int LORA_CTAS = 8;       // of a tile's cluster
-constexpr int LORA_TILE = 64;      // the most rows of a tile
+constexpr int LORA_TILE = 16;      // the most rows of a tile
 constexpr int LORA_MAX_RANK = 128;
 
 // Consecutive entries of LoraParams::rows, of one adapter (-1: none).
@@ -22,13 +21,17 @@ struct LoraParams {
   const LoraSlot* slots;     // [slots]
   const LoraTile* tiles;
   const int32_t* rows;       // rows in the order of the tiles
-  int n_tiles, tile_rows;    // tile_rows: 16, 32 or 64, the most that a tile has
+  int n_tiles;
   int n_in, n_out;           // n_in a multiple of 32
   int stride;                // ranks kept of each adapter, those past its own zero: lora_stride(max rank)
 };
 
-// Ranks as they are stored: whole steps of the products.
-inline int lora_stride(int max_rank) { return max_rank <= 16 ? 16 : (max_rank + 31) / 32 * 32; }
-cudaError_t lora_apply(const LoraParams& p, cudaStream_t s);
+// Ranks as they are stored: 16, 32, 64 or 128.
+inline int lora_stride(int max_rank) {
+  int r = 16;
+  while (r < max_rank) r *= 2;
+  return r;
+}
+cudaError_t lora_apply(const LoraParams& p, int sm_count, cudaStream_t s);
 
 }  // namespace kc

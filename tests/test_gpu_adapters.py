@@ -1,6 +1,6 @@
 """Low-rank adapters beside a projection against the formula in 64 bits. The result is rounded to bf16 once: half a step of its value
 (2^-8 of it at the most), and the fp32 sums before that: a term of A x or B t is off by 2^-24 of the sum of their absolute values
-for each of the additions, t loses 2^-17 as two bf16 numbers."""
+for each of the additions, and t = A x, scaled, goes into the second product as a bf16 number: off by half a step, 2^-8 of it at the most."""
 import numpy as np
 import pytest
 import torch
@@ -38,7 +38,7 @@ def formula(parts, x, y, slots):
             t, t_abs = v @ a.T, v.abs() @ a.abs().T
             out[rows] += scale * (t @ b.T)
             n_in, rank = a.shape[1], a.shape[0]
-            off[rows] = abs(scale) * ((t_abs * (n_in * 2.0 ** -24)) @ b.abs().T + t.abs() @ b.abs().T * (2.0 ** -17 + (2 * rank + 2) * 2.0 ** -24))
+            off[rows] = abs(scale) * ((t_abs * (n_in * 2.0 ** -24)) @ b.abs().T + t.abs() @ b.abs().T * (2.0 ** -8 + (2 * rank + 2) * 2.0 ** -24))
     return out, off
 
 
