@@ -162,7 +162,7 @@ struct Layer {
 
 // Per-step metadata, packed on the host and copied to the device in one transfer.
 struct MetaLayout {
-  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, sampling, uniform, prefix_units, rest_units, total;
+  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, sampling, uniform, shared_units, total;
 };
 
 struct kc_model {
@@ -193,10 +193,9 @@ struct kc_model {
   float* argmax_scratch = nullptr;     // per-CTA bests + counter of the fused reduction / arg-max of a streamed head
   float* partial_gu = nullptr;         // gate_up's fp32 partials while a gated down projection reads them (stream lane on)
   float* attn_ws = nullptr; size_t attn_ws_bytes = 0;
-  // Query maps of ptr [rows tokens], boxes of `box` and ATT_SMALL_TOKENS tokens: of a step's own units, and of the two launches of
-  // one that reads shared prefixes once.
+  // Query maps of ptr [rows tokens], boxes of `box` and ATT_SMALL_TOKENS tokens: of a step's own units, and of those over shared prefixes.
   struct QMaps { CUtensorMap map, small; const void* ptr = nullptr; int box = 0, rows = 0, gqa = 0; };
-  QMaps q_maps[3];
+  QMaps q_maps[2];
   float* tp_buf = nullptr;             // fp32 staging for the tensor-parallel all-reduce
   // Tensor-parallel exchange over peer memory (kc_tp_export / kc_tp_attach): the o_proj / down_proj output of exchange e
   // goes to tp_out[e & 1]; tp_flags[r] = the last exchange rank r has published. peer_* = every rank's buffers as
@@ -1231,12 +1230,11 @@ struct StepPlan {
   bool draws = false;              // sampled rows have settings and random numbers (kc_verify_step_sampled)
   std::vector<AttnUnit> units;
   // The same attention with the chunks that neighbours share read once (plan_shared): units of those chunks over the rows of all
-  // that share them, and units of the other chunks. One launch of all units, in `rest`, where one kernel takes both.
+  // that share them, and units of the other chunks.
   struct Shared {
-    bool on = false;
-    std::vector<AttnUnit> prefix, rest;
-    int prefix_tokens = 1, rest_tokens = 1;   // of an item
-    bool prefix_keys = false, rest_keys = false;
+    bool on = false, keys = false;
+    int tokens_per_item = 1;
+    std::vector<AttnUnit> units;
   } shared;
   MetaLayout lay{};
 };
@@ -1306,6 +1304,12 @@ std::vector<int> old_keys(kc_kv* kv, const kc_seq_step* seqs, int n_seqs) {
   return old;
 }
 
+// The widest run, in rows, with which a step over shared prefixes takes the kernel with a key per thread, for all its units. A call on its
+// own, attn_kernel -> attn_keys_kernel: 128 rows, 2048 keys shared by 32 sequences 30.0 -> 26.5 us, 64 and 8192 by 8 28.3 -> 23.3; 192
+// rows of 64 features, 4096 by 48 39.6 -> 39.3; 256, 6000 by 64 92 -> 100; 2560, 4096 by 64 132 -> 204; of 256 features 64 rows, 4096 by
+// 32 47.5 -> 40.2, 128 rows, 6144 by 16, capped 41.7 -> 51.2.
+int shared_key_rows(int head_dim) { return head_dim > 128 ? KEY_ROWS : 2 * KEY_ROWS; }
+
 // Units over shared prefixes. Sequences that stand next to each other in the step and name the same blocks for a chunk, and for
 // all chunks ahead of it, are a run there; no key of the chunk is written by the step. The run's rows are taken together against
 // the chunk, as many as a unit holds, and every chunk's partial result is merged in index order as ever: a row has the bits
@@ -1326,7 +1330,6 @@ void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& o
   }
   if (most == 0) return;
   int widest = 1;   // tokens of a run
-  long long rest_tiles = 0;
   auto runs = [&](int c, auto&& each) {
     for (int i = 0, j; i < n; i = j + 1) {
       for (j = i; j + 1 < n && common[j + 1] > c; ++j) {}
@@ -1334,42 +1337,35 @@ void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& o
     }
   };
   runs(0, [&](int, int r0, int r1) { widest = std::max(widest, r1 - r0); });
-  for (int i = 0; i < n; ++i) rest_tiles += (seqs[i].offset + seqs[i].len - std::max(common[i], common[i + 1]) * ATT_CHUNK + 127) / 128;
-  sh.rest_tokens = p->tokens_per_item;
-  sh.rest_keys = sh.rest_tokens * gqa <= attn_key_rows(head_dim, alone, capped, AttnForm::apart, rest_tiles * kv_heads, sm_count);
-  sh.prefix_keys = widest * gqa <= KEY_ROWS;
-  sh.prefix_tokens = std::min(std::max(1, (sh.prefix_keys ? KEY_ROWS : ATT_ROWS) / gqa), widest);
-  auto small = [](int box, int tokens) { return box > ATT_SMALL_TOKENS && tokens <= ATT_SMALL_TOKENS ? 1 : 0; };
-  const bool one_launch = sh.prefix_keys == sh.rest_keys;
-  if (one_launch) sh.prefix_tokens = sh.rest_tokens = std::max(sh.prefix_tokens, sh.rest_tokens);
+  sh.keys = p->tokens_per_item * gqa <= KEY_ROWS && widest * gqa <= shared_key_rows(head_dim);
+  sh.tokens_per_item = std::min(std::max(1, (sh.keys ? KEY_ROWS : ATT_ROWS) / gqa), std::max(widest, p->tokens_per_item));
+  auto small = [&](int tokens) { return sh.tokens_per_item > ATT_SMALL_TOKENS && tokens <= ATT_SMALL_TOKENS ? 1 : 0; };
   for (int c = 0; c < most; ++c)
     runs(c, [&](int i, int r0, int r1) {
-      for (int t = r0; t < r1; t += sh.prefix_tokens) {
+      for (int t = r0; t < r1; t += sh.tokens_per_item) {
         AttnUnit u{};
-        u.seq = i; u.tok0 = t; u.ntok = std::min(sh.prefix_tokens, r1 - t);
+        u.seq = i; u.tok0 = t; u.ntok = std::min(sh.tokens_per_item, r1 - t);
         u.pos0 = u.old = (c + 1) * ATT_CHUNK;   // every row lies past the chunk
         u.chunk0 = c; u.chunk1 = c + 1;
-        u.small = small(sh.prefix_tokens, u.ntok);
-        sh.prefix.push_back(u);
+        u.small = small(u.ntok);
+        sh.units.push_back(u);
       }
     });
-  std::vector<AttnUnit> full, last;
+  std::vector<AttnUnit> last;
   for (int i = 0; i < n; ++i)
     for (int t = 0; t < seqs[i].len; t += p->tokens_per_item) {
       AttnUnit u{};
       u.seq = i; u.tok0 = row[i] + t; u.ntok = std::min(p->tokens_per_item, seqs[i].len - t); u.pos0 = seqs[i].offset + t;
-      u.small = small(sh.rest_tokens, u.ntok);
+      u.small = small(u.ntok);
       u.old = old[i];
       const int end = (u.pos0 + u.ntok - 1) / ATT_CHUNK + 1;
       for (int c = std::max(common[i], common[i + 1]); c < end; ++c) {
         u.chunk0 = c; u.chunk1 = c + 1;
-        (c + 1 < end ? full : last).push_back(u);
+        (c + 1 < end ? sh.units : last).push_back(u);
       }
     }
   std::stable_sort(last.begin(), last.end(), [](const AttnUnit& a, const AttnUnit& b) { return (a.pos0 + a.ntok - 1) % ATT_CHUNK > (b.pos0 + b.ntok - 1) % ATT_CHUNK; });
-  if (one_launch) sh.rest.swap(sh.prefix);
-  sh.rest.insert(sh.rest.end(), full.begin(), full.end());
-  sh.rest.insert(sh.rest.end(), last.begin(), last.end());
+  sh.units.insert(sh.units.end(), last.begin(), last.end());
   sh.on = true;
 }
 
@@ -1425,7 +1421,7 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
   L.v_draft = put((size_t)n * 4);
   L.feed = put((size_t)n * 4);
   if (p.draws) { L.sampling = put((size_t)p.n_sampled * sizeof(kc_sampling)); L.uniform = put((size_t)p.n_sampled * 4); }
-  if (p.shared.on) { L.prefix_units = put(p.shared.prefix.size() * sizeof(AttnUnit)); L.rest_units = put(p.shared.rest.size() * sizeof(AttnUnit)); }
+  if (p.shared.on) L.shared_units = put(p.shared.units.size() * sizeof(AttnUnit));
   L.total = at;
   *plan = std::move(p);
   return KC_OK;
@@ -1458,10 +1454,8 @@ int upload_meta(kc_model* m, kc_kv* kv, const uint32_t* token_ids, const kc_seq_
   int32_t* slotv = reinterpret_cast<int32_t*>(hbuf + L.kv_slot);
   int32_t* sampled = reinterpret_cast<int32_t*>(hbuf + L.sampled);
   int32_t* tables = reinterpret_cast<int32_t*>(hbuf + L.tables);
-  auto put_units = [&](size_t to, const std::vector<AttnUnit>& u) { if (!u.empty()) memcpy(hbuf + to, u.data(), u.size() * sizeof(AttnUnit)); };
-  put_units(L.units, p.units);
-  put_units(L.prefix_units, p.shared.prefix);
-  put_units(L.rest_units, p.shared.rest);
+  memcpy(hbuf + L.units, p.units.data(), p.units.size() * sizeof(AttnUnit));
+  if (p.shared.on) memcpy(hbuf + L.shared_units, p.shared.units.data(), p.shared.units.size() * sizeof(AttnUnit));
   int32_t* v_row = reinterpret_cast<int32_t*>(hbuf + L.v_row_off);
   int32_t* v_doff = reinterpret_cast<int32_t*>(hbuf + L.v_draft_off);
   int32_t* v_dlen = reinterpret_cast<int32_t*>(hbuf + L.v_draft_len);
@@ -1527,7 +1521,7 @@ AttnParams attn_params(kc_model* m, kc_kv* kv, const StepPlan& p, int layer, bf1
   a.Hq = Hq; a.Hkv = kv->kv_heads; a.gqa = Hq / kv->kv_heads;
   a.layer = layer; a.NB = kv->num_blocks; a.BS = kv->block_size;
   a.max_chunks = p.max_chunks;
-  a.whole = p.whole ? 1 : 0; a.single = p.max_chunks == 1 ? 1 : 0; a.keys = p.keys ? 1 : 0; a.merge = 1;
+  a.whole = p.whole ? 1 : 0; a.single = p.max_chunks == 1 ? 1 : 0; a.keys = p.keys ? 1 : 0;
   a.scale = scale; a.softcap = softcap; a.window = window;
   a.q_tokens = p.tokens_per_item;
   a.kv5d = kv->map5d ? 1 : 0;
@@ -1546,9 +1540,7 @@ int ensure_q_map(kc_model* m, kc_model::QMaps* q, const bf16* ptr, int rows, int
 }
 int ensure_q_maps(kc_model* m, const bf16* q, int rows, int Hq, int gqa, const StepPlan& p) {
   RC(ensure_q_map(m, &m->q_maps[0], q, rows, Hq, gqa, p.tokens_per_item));
-  if (!p.shared.on) return KC_OK;
-  RC(ensure_q_map(m, &m->q_maps[1], q, rows, Hq, gqa, p.shared.rest_tokens));
-  return p.shared.prefix.empty() ? KC_OK : ensure_q_map(m, &m->q_maps[2], q, rows, Hq, gqa, p.shared.prefix_tokens);
+  return p.shared.on ? ensure_q_map(m, &m->q_maps[1], q, rows, Hq, gqa, p.shared.tokens_per_item) : KC_OK;
 }
 
 // One layer's attention of a step whose maps and workspace are there. Every row of a windowed layer has a mask of its own, so
@@ -1556,23 +1548,17 @@ int ensure_q_maps(kc_model* m, const bf16* q, int rows, int Hq, int gqa, const S
 int run_attention(kc_model* m, kc_kv* kv, const StepPlan& p, int layer, bf16* out, float scale, float softcap, int window, int Hq, bool in_order) {
   kc_ctx* c = m->ctx;
   AttnParams a = attn_params(m, kv, p, layer, out, scale, softcap, window, Hq);
-  auto launch = [&](const kc_model::QMaps& q, int launches, bool ordered) -> int {
-    LAUNCH(c, KC_PROF_ATTN, launches, paged_attention(kv->map, kv->map_one, q.map, q.small, a, ordered, kv->head_dim, p.n, c->sm_count, c->stream));
-    return KC_OK;
-  };
-  if (!p.shared.on || window > 0) return launch(m->q_maps[0], p.whole || p.max_chunks == 1 ? 1 : 2, in_order);
-  a.whole = a.single = 0;
-  const bool two = !p.shared.prefix.empty();
-  if (two) {
-    a.units = reinterpret_cast<const AttnUnit*>(m->meta_dev + p.lay.prefix_units);
-    a.n_units = (int)p.shared.prefix.size();
-    a.q_tokens = p.shared.prefix_tokens; a.keys = p.shared.prefix_keys ? 1 : 0; a.merge = 0;
-    RC(launch(m->q_maps[2], 1, in_order));
+  const bool shared = p.shared.on && window <= 0;
+  if (shared) {
+    a.units = reinterpret_cast<const AttnUnit*>(m->meta_dev + p.lay.shared_units);
+    a.n_units = (int)p.shared.units.size();
+    a.q_tokens = p.shared.tokens_per_item; a.keys = p.shared.keys ? 1 : 0;
+    a.whole = a.single = 0;
   }
-  a.units = reinterpret_cast<const AttnUnit*>(m->meta_dev + p.lay.rest_units);
-  a.n_units = (int)p.shared.rest.size();
-  a.q_tokens = p.shared.rest_tokens; a.keys = p.shared.rest_keys ? 1 : 0; a.merge = 1;
-  return launch(m->q_maps[1], 2, in_order && !two);
+  const kc_model::QMaps& q = m->q_maps[shared ? 1 : 0];
+  LAUNCH(c, KC_PROF_ATTN, a.whole || a.single ? 1 : 2,
+         paged_attention(kv->map, kv->map_one, q.map, q.small, a, in_order, kv->head_dim, p.n, c->sm_count, c->stream));
+  return KC_OK;
 }
 
 // Brings every tensor-parallel rank's bf16 [n, H] sublayer output to every rank: out[r] = rank r's rows. The SUM is

@@ -662,7 +662,7 @@ cudaError_t launch_d(const CUtensorMap& map, const CUtensorMap& kmap, const CUte
     }
     e = launch_attn<D, false>(map, q, q_small, p, in_order, sm_count, s);
   }
-  if (e != cudaSuccess || p.single || !p.merge) return e;
+  if (e != cudaSuccess || p.single) return e;
   const int n_rows = n_tokens * p.Hq;
   return launch_k(attn_combine_kernel<D>, dim3((n_rows + 7) / 8), dim3(256), 0, s, p, n_rows);
 }

@@ -34,7 +34,6 @@ struct AttnParams {
   int layer, NB, BS;
   int max_chunks;
   int whole;                   // 1: every unit holds all chunks of its rows: the kernel writes `out`, no combine kernel follows
-  int merge;                   // 0: another launch of the same rows follows, whose combine kernel merges what both leave
   int single;                  // 1: no row of the step has a second chunk (max_chunks == 1): no combine kernel either
   float scale;                 // softmax scale (applied to fp32 scores)
   float softcap;               // 0 = off
