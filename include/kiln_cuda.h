@@ -440,8 +440,9 @@ KC_API int kc_paged_attention(kc_ctx_t ctx, kc_kv_t kv, int32_t layer, const voi
 
 /* The attention of a step as a handle, for callers that run it layer by layer, and for batches that share a long prefix: blocks
  * that sequences standing next to each other in `seqs` name at the same places of their tables, from the start on, are read
- * once for the rows of all of them, in pieces of 512 keys; what follows is each one's own. A row has the bits that
- * kc_paged_attention gives it. The plan holds the step's description (seqs and their tables are copied; sample_rows are not
+ * once for the rows of all of them, in pieces of 512 keys, where that saves enough (a model's own steps do the same); what
+ * follows is each one's own. A row has the bits that kc_paged_attention gives it. kc_attn_plan_keys: keys that the plan reads for
+ * a kv head of a layer without a window, and keys that it would read for every sequence apart. The plan holds the step's description (seqs and their tables are copied; sample_rows are not
  * looked at) and a workspace; it belongs to the pools' context and is freed before the pools. kc_attn_plan_run takes q bf16
  * [n, num_heads, head_dim] post-RoPE, n the sum of the lens, and writes out bf16 [n, num_heads*head_dim], both 16-byte aligned; scale, softcap and
  * window as in kc_paged_attention (a layer with a window reads every sequence's keys for itself). It expects the step's K/V in
@@ -450,6 +451,7 @@ KC_API int kc_paged_attention(kc_ctx_t ctx, kc_kv_t kv, int32_t layer, const voi
 typedef struct kc_attn_plan* kc_attn_plan_t;
 KC_API int kc_attn_plan_create(kc_ctx_t ctx, kc_kv_t kv, const kc_seq_step* seqs, int32_t n_seqs, int32_t num_heads,
                                kc_attn_plan_t* out);
+KC_API int kc_attn_plan_keys(kc_attn_plan_t plan, int64_t* read, int64_t* apart);
 KC_API void kc_attn_plan_free(kc_attn_plan_t plan);
 KC_API int kc_attn_plan_run(kc_attn_plan_t plan, int32_t layer, const void* q_dev, float scale, float softcap,
                             int32_t window, void* out_dev);

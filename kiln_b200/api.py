@@ -782,7 +782,7 @@ def paged_attention(ctx: Context, kv: PagedKv, layer: int, q: torch.Tensor, seqs
 
 class AttentionPlan:
     """The paged attention of one step, planned once and run for each layer (kc_attn_plan_create). Blocks at the start of the
-    tables that neighbouring sequences share are read once for all of them; a row has paged_attention's bits."""
+    tables that neighbouring sequences share are read once for all of them where that saves enough; a row has paged_attention's bits."""
 
     def __init__(self, ctx: Context, kv: PagedKv, heads: int, seqs: Sequence[SeqStep]):
         self.ctx, self.kv, self.heads = ctx, kv, heads
@@ -791,6 +791,12 @@ class AttentionPlan:
         p = _PackedStep(StepBatch([], seqs))
         check(L.lib().kc_attn_plan_create(ctx._h, kv._h, p.seq_arr, p.n_seqs, heads, C.byref(self._h)))
         ctx._adopt(self)
+
+    def keys(self):
+        """(keys read for a kv head of a layer, keys that reading every sequence apart would take): equal where nothing is shared."""
+        read, apart = C.c_int64(0), C.c_int64(0)
+        check(L.lib().kc_attn_plan_keys(self._h, C.byref(read), C.byref(apart)))
+        return int(read.value), int(apart.value)
 
     def run(self, layer: int, q: torch.Tensor, scale: float, softcap: float = 0.0, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q bf16 [tokens, heads, head_dim] post-RoPE → bf16 [tokens, heads*head_dim], part of torch's current stream

@@ -76,20 +76,20 @@ def run_both(ctx, kv, data, heads, seqs, seed, softcap=0.0, scale=None, layer=0,
 
 
 HEADS = [(32, 8, 128), (28, 4, 128), (32, 8, 64), (16, 8, 256), (8, 8, 128), (24, 1, 64), (64, 1, 128)]
-SHARED = {
-    "two of one chunk": [(512, [(1, 512), (1, 600)])],
-    "one chunk, ends on its edge": [(512, [(1, 511), (1, 512), (1, 513)])],       # the first one's own row stands in the chunk: not shared with it
-    "not a block's multiple": [(1001, [(1, 1001), (1, 1030), (1, 1500)])],
-    "verify rows": [(1024, [(5, 1300)] * 9)],
-    "ragged rows": [(1536, [(3, 1600), (1, 1536), (6, 2100), (2, 1700), (40, 1550)])],
-    "many": [(1100, [(1, 1100 + 7 * i) for i in range(70)])],
-    "two groups and loners": [(0, [(1, 700)]), (1024, [(1, 1100), (2, 1024)]), (0, [(1, 3), (1, 0)]), (2048, [(1, 2050), (1, 3000), (1, 2048)])],
-    "nothing shared": [(0, [(1, 900), (1, 800)])],
-    "shared below a chunk": [(496, [(1, 900), (1, 800)])],
-    "alone": [(2000, [(4, 2040)])],
-    "no history": [(0, [(1, 0)])],
-    "a piece of a prompt behind a shared prefix": [(1024, [(130, 1024), (1, 1200), (1, 1300)])],
+SHARED = {   # what 30 to 150 sequences share; enough for it to be read once with a kv head alone too
+    "whole chunks": [(2048, [(1, 2048 + i) for i in range(80)])],
+    "ends on its edge": [(1536, [(1, 1535 + i % 3) for i in range(150)])],          # the ones whose own row stands in the last chunk don't share it
+    "not a block's multiple": [(2001, [(1, 2001 + 29 * i) for i in range(90)])],
+    "verify rows": [(1600, [(5, 1700 + i) for i in range(70)])],
+    "ragged rows": [(2560, [(1 + i % 6, 2600 + 61 * i) for i in range(60)])],
+    "two groups and loners": [(0, [(1, 700)]), (2048, [(1, 2100 + i) for i in range(60)]), (0, [(1, 3), (1, 0), (2, 1500)]), (3000, [(1 + i % 2, 3050 + 40 * i) for i in range(50)])],
+    "few": [(8192, [(1, 8200 + i) for i in range(30)])],
 }
+
+
+def shares(plan):
+    read, apart = plan.keys()
+    return read < apart
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
@@ -98,53 +98,77 @@ def test_rows_have_the_bits_that_they_have_alone(ctx, heads, kv_heads, dim, name
     seqs, total = tables(SHARED[name], 16, len(name))
     kv, data = pools(ctx, kv_heads, dim, total, 16, 5)
     softcap = 30.0 if dim == 256 else 0.0
-    q, got, _ = run_both(ctx, kv, data, heads, seqs, 7, softcap)
+    q, got, plan = run_both(ctx, kv, data, heads, seqs, 7, softcap)
+    # with 24 heads to a kv head and more, several rows of one sequence fill a unit by themselves
+    assert shares(plan) or (heads // kv_heads >= 24 and any(s.len > 1 for s in seqs))
     close(got, formula(data[0], q, seqs, dim ** -0.5, softcap))
     assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("groups", [
+    [(512, [(1, 512), (1, 600)])], [(0, [(1, 900), (1, 800)])], [(496, [(1, 900 + i) for i in range(200)])], [(2000, [(4, 2040)])], [(0, [(1, 0)])],
+    [(1024, [(130, 1024)] + [(1, 1200 + i) for i in range(90)])]])
+def test_what_is_not_shared(ctx, groups):
+    """Too little to be read once, less than a chunk, one sequence, no history, beside a piece of a prompt."""
+    seqs, total = tables(groups, 16, 1)
+    kv, data = pools(ctx, 4, 128, total, 16, 5)
+    q, got, plan = run_both(ctx, kv, data, 16, seqs, 7)
+    assert not shares(plan)
+    close(got, formula(data[0], q, seqs, 128 ** -0.5, 0.0))
 
 
 @pytest.mark.parametrize("block_size", [16, 32, 64, 128])
 @pytest.mark.parametrize("softcap,scale", [(0.0, None), (20.0, None), (0.0, -0.1), (0.0, 0.0), (5.0, 3.0)])
 def test_block_sizes_caps_and_scales(ctx, block_size, softcap, scale):
-    seqs, total = tables([(1024, [(2, 1100 + 130 * i) for i in range(6)])], block_size, 3)
+    seqs, total = tables([(2048, [(2, 2100 + 11 * i) for i in range(50)])], block_size, 3)
     kv, data = pools(ctx, 2, 128, total, block_size, 9)
-    run_both(ctx, kv, data, 8, seqs, 1, softcap, scale)
+    _, _, plan = run_both(ctx, kv, data, 8, seqs, 1, softcap, scale)
+    assert shares(plan)
 
 
 def test_a_tree_of_prefixes(ctx):
-    """All share a chunk, pairs three, and the middle ones another two: every chunk goes by who has it in common."""
+    """All share two chunks, eights of them two more, and some in the middle another one: every chunk goes by who has it in common."""
     bs, rng = 16, np.random.default_rng(2)
-    per, order = 32, np.random.default_rng(2).permutation(2000)
-    trunk, branches, at, seqs = order[:per], [order[per * (1 + 2 * i): per * (3 + 2 * i)] for i in range(4)], 1000, []
-    deeper = order[per * 10: per * 12]
-    for i in range(8):
-        off = 512 + 1024 + (1024 if i in (3, 4, 5) else 0) + int(rng.integers(0, 300))
-        head = [trunk, branches[i // 2]] + ([deeper] if i in (3, 4, 5) else [])
-        head = np.concatenate(head)
+    order = np.random.default_rng(2).permutation(4000)
+    trunk, branches, deeper, at, seqs = order[:64], [order[64 * (1 + i): 64 * (2 + i)] for i in range(8)], order[640:672], 700, []
+    for i in range(64):
+        deep = 20 <= i < 40
+        head = np.concatenate([trunk, branches[i // 8]] + ([deeper] if deep else []))
+        off = len(head) * bs + int(rng.integers(0, 300))
         n = -(-(off + 1 + i % 3) // bs)
         own = order[at: at + n - len(head)]
         at += len(own)
         seqs.append(api.SeqStep(1 + i % 3, off, 0, np.concatenate([head, own]).astype(np.uint32)))
-    kv, data = pools(ctx, 4, 128, 2000, bs, 4)
-    q, got, _ = run_both(ctx, kv, data, 16, seqs, 3)
+    kv, data = pools(ctx, 4, 128, 4000, bs, 4)
+    q, got, plan = run_both(ctx, kv, data, 16, seqs, 3)
+    # 64 tables share 1024 keys, read by units of 32 of their 127 tokens; eights 1024 more; 20 in the middle 512 in three runs, which
+    # their branches' edges cut
+    read, apart = plan.keys()
+    assert apart - read == 1024 * (64 - 4) + 1024 * (64 - 8) + 512 * (20 - 3)
     close(got, formula(data[0], q, seqs, 128 ** -0.5, 0.0))
 
 
-def test_one_table_for_all(ctx):
-    """Every block is shared, the rows' own among them, at different positions."""
-    kv, data = pools(ctx, 2, 128, 80, 16, 4)
-    table = np.random.default_rng(0).permutation(80).astype(np.uint32)
-    seqs = [api.SeqStep(3, off, 0, table) for off in (1000, 1024, 1100, 40, 600, 1277)]
-    q, got, _ = run_both(ctx, kv, data, 8, seqs, 3)
+@pytest.mark.parametrize("early", [False, True])
+def test_one_table_for_all(ctx, early):
+    """Every block is shared, the rows' own among them, at different positions. Where one of them is written in a shared chunk nothing behind
+    it is read for all."""
+    kv, data = pools(ctx, 2, 128, 160, 16, 4)
+    table = np.random.default_rng(0).permutation(160).astype(np.uint32)
+    seqs = [api.SeqStep(3, 2000 + 8 * i, 0, table) for i in range(65)]
+    if early:
+        seqs += [api.SeqStep(3, off, 0, table) for off in (40, 600)]
+    q, got, plan = run_both(ctx, kv, data, 8, seqs, 3)
+    assert shares(plan) != early
     close(got, formula(data[0], q, seqs, 128 ** -0.5, 0.0))
 
 
 def test_windows_layers_streams_and_graphs(ctx):
     """A plan serves all layers, windowed ones too, on whatever stream is the current one, and in a graph that is replayed after
     the queries and the pools have changed."""
-    seqs, total = tables([(1024, [(2, 1030 + 50 * i) for i in range(7)])], 16, 1)
+    seqs, total = tables([(2048, [(2, 2060 + 20 * i) for i in range(50)])], 16, 1)
     kv, data = pools(ctx, 2, 128, total, 16, 4, layers=2)
     q, got, plan = run_both(ctx, kv, data, 8, seqs, 3, layer=1)
+    assert shares(plan)
     scale = 128 ** -0.5
     for window in (1, 100, 600, 5000):
         w = plan.run(0, q, scale, 0.0, window)
@@ -177,20 +201,55 @@ def test_windows_layers_streams_and_graphs(ctx):
 
 def test_large_scores(ctx):
     """One key outweighs all others by far: maxima that move by thousands of binary orders from chunk to chunk."""
-    seqs, total = tables([(512, [(1, 520), (1, 700), (2, 512)])], 16, 1)
+    seqs, total = tables([(2048, [(1, 2060 + 9 * i) for i in range(80)])], 16, 1)
     kv, data = pools(ctx, 2, 64, total, 16, 4, std=40.0)
-    q, got, _ = run_both(ctx, kv, data, 8, seqs, 3, std=40.0)
+    q, got, plan = run_both(ctx, kv, data, 8, seqs, 3, std=40.0)
+    assert shares(plan)
     close(got, formula(data[0], q, seqs, 64 ** -0.5, 0.0))
 
 
 def test_rows_past_the_shared_ones_are_left(ctx):
-    seqs, total = tables([(512, [(1, 512)] * 3)], 16, 1)
+    seqs, total = tables([(2048, [(1, 2048)] * 90)], 16, 1)
     kv, data = pools(ctx, 2, 64, total, 16, 4)
-    q = torch.randn(3, 8, 64, device="cuda").to(torch.bfloat16)
-    out = torch.full((5, 512), 7.0, dtype=torch.bfloat16, device="cuda")
-    api.AttentionPlan(ctx, kv, 8, seqs).run(0, q, 0.125, out=out[1:4])
+    q = torch.randn(90, 8, 64, device="cuda").to(torch.bfloat16)
+    out = torch.full((92, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    plan = api.AttentionPlan(ctx, kv, 8, seqs)
+    assert shares(plan)
+    plan.run(0, q, 0.125, out=out[1:91])
     torch.cuda.synchronize()
-    assert (out[0] == 7).all() and (out[4] == 7).all() and torch.equal(out[1:4], api.paged_attention(ctx, kv, 0, q, seqs, 0.125))
+    assert (out[0] == 7).all() and (out[91] == 7).all() and torch.equal(out[1:91], api.paged_attention(ctx, kv, 0, q, seqs, 0.125))
+
+
+def test_a_models_steps_share(ctx):
+    """A model's verify step over sequences that share a prompt: the logits of a sequence are those it has alone, bit for bit, and
+    the K/V it writes too; sampled tokens and counts follow."""
+    cfg = PRESETS["tiny-llama-d128"]
+    model = api.CudaModel(ctx, cfg, synth_checkpoint(cfg, seed=1), max_step_tokens=512, max_step_seqs=128)
+    rng, n, shared = np.random.default_rng(1), 100, 1040
+    kv = api.PagedKv(ctx, model.kv_spec(65 + 4 * n + 4, 16))
+    prompt = rng.integers(0, cfg.vocab_size, 1040).tolist()
+    for at in range(0, shared, 512):
+        piece = prompt[at: at + 512]
+        model.forward_step(api.StepBatch(piece, [api.SeqStep(len(piece), at, 0, np.arange(65, dtype=np.uint32))]), kv)
+    own = [np.arange(65 + 4 * i, 69 + 4 * i, dtype=np.uint32) for i in range(n)]
+    ids = rng.integers(0, cfg.vocab_size, (n, 3))
+    seqs = [api.SeqStep(3, shared, 3, np.concatenate([np.arange(65, dtype=np.uint32), own[i]])) for i in range(n)]
+    plan = api.AttentionPlan(ctx, kv, cfg.num_attention_heads, seqs)
+    assert shares(plan)
+    batch = api.StepBatch(ids.reshape(-1).tolist(), seqs)
+    logits = model.forward_step(batch, kv)
+    ctx.sync()
+    together = logits.clone()
+    wrote = kv.read_block_bytes(int(own[7][0]))
+    for i in (0, 7, 50, 99):
+        kv.copy_block(68 + 4 * n - 1, int(own[i][0]))      # what it wrote is written again
+        alone = model.forward_step(api.StepBatch(ids[i].tolist(), [seqs[i]]), kv)
+        ctx.sync()
+        assert torch.equal(alone.view(torch.int16), together[3 * i: 3 * i + 3].view(torch.int16))
+    assert kv.read_block_bytes(int(own[7][0])) == wrote
+    rows, ncom, nacc = model.verify_step(batch, kv)
+    assert torch.equal(torch.from_numpy(rows.astype(np.int64)).cuda(), api.greedy_rows(ctx, together).long())
+    assert ctx.device_status() == 0
 
 
 def test_refusals(ctx):
