@@ -164,6 +164,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
   clear_bins();
   for (int i = tid; i < DRAW_RUNS * 32; i += DRAW_THREADS) { s.mass[0][i] = 0.0; s.count[0][i] = 0; }
   if (tid == 0) s.above = 0;
+  __syncthreads();                       // the bins are clear before any thread counts: the arrival above says nothing about them
   cluster_wait();
   pdl_wait();
   const DrawSetting set = settings[row_index];

@@ -161,6 +161,21 @@ def test_rows_do_not_hang_on_their_number(ctx):
         assert torch.equal(got, want[:n]) and torch.equal(q.view(torch.int32), p[:n].view(torch.int32))
 
 
+@pytest.mark.parametrize("rows,vocab", [(310, 50001), (310, 4099), (90, 4099), (40, 257), (1, 8)])
+def test_every_run_counts_every_token(ctx, rows, vocab):
+    """The same rows many times over: a token that one run did not count would show in the log probability."""
+    logits = language(rows, vocab, 5)
+    params = api.pack_sampling([api.SamplingParams()] * rows, logits.device)
+    u = torch.rand(rows, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    first = [t.clone() for t in api.sample_rows(ctx, logits, params, u)]
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(400):
+        tokens, logprobs = api.sample_rows(ctx, logits, params, u)
+        wrong += (tokens != first[0]).sum() + (logprobs != first[1]).sum()
+    assert int(wrong) == 0
+    check(ctx, logits[:5], [(1.0, 0, 1.0, 0.0)] * min(rows, 5), u[:5].tolist())
+
+
 def test_streams_and_graphs(ctx):
     """Part of whatever stream is torch's current one, of the context's own, and of a graph that is replayed with new rows."""
     x, u = language(5, 4099, 1), torch.tensor([0.1, 0.4, 0.6, 0.8, 0.95], device="cuda")
