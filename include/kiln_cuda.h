@@ -397,8 +397,9 @@ KC_API int kc_quantized_matmul_static(kc_ctx_t ctx, kc_qweight_t w, const void* 
 KC_API int64_t kc_static_scratch_bytes(void);
 
 /* Low-rank adapters of many requests beside one projection (no counterpart in the reference): out_i = y_i + scale_a B_a (A_a x_i)
- * for every row i, a being the adapter of its request; rows without one keep their y. A x, scale and the sums are in fp32, y is
- * the projection's bf16 output (kc_quantized_matmul), the result is rounded to bf16 once.
+ * for every row i, a being the adapter of its request; rows without one keep their y. Sums and scale are in fp32; A x is rounded to
+ * bf16 between the two products, as an operand of the second; y is the projection's bf16 output (kc_quantized_matmul), and the
+ * result is rounded to bf16.
  * kc_adapters_create makes the adapters of one projection: `slots` of them, of ranks up to max_rank (1..128), empty to begin with; in_features a
  * multiple of 32. kc_adapters_set copies A bf16 [rank, in] and B bf16 [out, rank] into a slot, in place of what it held
  * (rank 0 empties it; a and b may then be NULL); it returns when the copies are done, behind everything queued before it. */
@@ -413,7 +414,7 @@ KC_API void kc_adapters_free(kc_adapters_t adapters);
  * rows of one request best stand together. */
 KC_API int kc_adapter_rows_create(kc_ctx_t ctx, const int32_t* slot_of_row, int32_t m, kc_adapter_rows_t* out);
 KC_API void kc_adapter_rows_free(kc_adapter_rows_t rows);
-/* x bf16 [m, in], 16-byte aligned; y and out bf16 [m, out], the same buffer or apart. A slot that the rows name and
+/* x bf16 [m, in], 16-byte aligned; y and out bf16 [m, out], the same buffer or apart; out apart from x. A slot that the rows name and
  * the adapters do not have is refused. Asynchronous on the context's stream; no workspace, so that it may be captured and
  * several may run at once. */
 KC_API int kc_adapters_apply(kc_adapters_t adapters, kc_adapter_rows_t rows, const void* x_dev, const void* y_dev,
@@ -441,16 +442,20 @@ KC_API int kc_paged_attention(kc_ctx_t ctx, kc_kv_t kv, int32_t layer, const voi
 /* The attention of a step as a handle, for callers that run it layer by layer, and for batches that share a long prefix: blocks
  * that sequences standing next to each other in `seqs` name at the same places of their tables, from the start on, are read
  * once for the rows of all of them, in pieces of 512 keys, where that saves enough (a model's own steps do the same); what
- * follows is each one's own. A row has the bits that kc_paged_attention gives it. kc_attn_plan_keys: keys that the plan reads for
- * a kv head of a layer without a window, and keys that it would read for every sequence apart. The plan holds the step's description (seqs and their tables are copied; sample_rows are not
- * looked at) and a workspace; it belongs to the pools' context and is freed before the pools. kc_attn_plan_run takes q bf16
- * [n, num_heads, head_dim] post-RoPE, n the sum of the lens, and writes out bf16 [n, num_heads*head_dim], both 16-byte aligned; scale, softcap and
- * window as in kc_paged_attention (a layer with a window reads every sequence's keys for itself). It expects the step's K/V in
- * the pools by the time it runs, is asynchronous on the context's stream and may be captured. Runs of one plan share its
- * workspace: one after the other. */
+ * follows is each one's own. A row has the bits that kc_paged_attention gives it. The plan holds the step's description (seqs
+ * and their tables are copied; sample_rows are not looked at) and a workspace; it belongs to the pools' context and is freed
+ * before the pools. kc_attn_plan_set puts another step of the same heads and pools in its place, behind the runs queued before it,
+ * and allocates only what the plan does not have yet: one plan serves a generation step after step. It is refused once a
+ * graph has been captured over a run. kc_attn_plan_keys: keys that the plan reads for a kv head of a layer without a window,
+ * and keys that it would read for every sequence apart. kc_attn_plan_run takes q bf16 [n, num_heads, head_dim] post-RoPE, n
+ * the sum of the lens, and writes out bf16 [n, num_heads*head_dim], both 16-byte aligned and apart; scale, softcap and window
+ * as in kc_paged_attention (a layer with a window reads every sequence's keys for itself). It expects the step's K/V in the
+ * pools by the time it runs, is asynchronous on the context's stream and may be captured. Runs of one plan share its
+ * workspace: one after the other, graphs that hold them too. */
 typedef struct kc_attn_plan* kc_attn_plan_t;
 KC_API int kc_attn_plan_create(kc_ctx_t ctx, kc_kv_t kv, const kc_seq_step* seqs, int32_t n_seqs, int32_t num_heads,
                                kc_attn_plan_t* out);
+KC_API int kc_attn_plan_set(kc_attn_plan_t plan, const kc_seq_step* seqs, int32_t n_seqs);
 KC_API int kc_attn_plan_keys(kc_attn_plan_t plan, int64_t* read, int64_t* apart);
 KC_API void kc_attn_plan_free(kc_attn_plan_t plan);
 KC_API int kc_attn_plan_run(kc_attn_plan_t plan, int32_t layer, const void* q_dev, float scale, float softcap,

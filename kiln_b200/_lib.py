@@ -111,6 +111,7 @@ _SIGNATURES = {
     "kc_paged_attention": (C.c_int, [_P, _P, C.c_int32, _P, C.c_int32, C.c_int32, C.POINTER(KcSeqStep), C.c_int32,
                                      C.c_float, C.c_float, C.c_int32, _P]),
     "kc_attn_plan_create": (C.c_int, [_P, _P, C.POINTER(KcSeqStep), C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "kc_attn_plan_set": (C.c_int, [_P, C.POINTER(KcSeqStep), C.c_int32]),
     "kc_attn_plan_keys": (C.c_int, [_P, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "kc_attn_plan_free": (None, [_P]),
     "kc_attn_plan_run": (C.c_int, [_P, C.c_int32, _P, C.c_float, C.c_float, C.c_int32, _P]),

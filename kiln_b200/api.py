@@ -787,10 +787,17 @@ class AttentionPlan:
     def __init__(self, ctx: Context, kv: PagedKv, heads: int, seqs: Sequence[SeqStep]):
         self.ctx, self.kv, self.heads = ctx, kv, heads
         self._h = C.c_void_p()
-        self.tokens = sum(s.len for s in seqs)
         p = _PackedStep(StepBatch([], seqs))
         check(L.lib().kc_attn_plan_create(ctx._h, kv._h, p.seq_arr, p.n_seqs, heads, C.byref(self._h)))
+        self.tokens = sum(s.len for s in seqs)
         ctx._adopt(self)
+
+    def set(self, seqs: Sequence[SeqStep]) -> None:
+        """Another step in the plan's place, behind the runs queued before: a generation keeps one plan and sets it every step.
+        Refused once a graph has been captured over a run."""
+        p = _PackedStep(StepBatch([], seqs))
+        check(L.lib().kc_attn_plan_set(self._h, p.seq_arr, p.n_seqs))
+        self.tokens = sum(s.len for s in seqs)
 
     def keys(self):
         """(keys read for a kv head of a layer, keys that reading every sequence apart would take): equal where nothing is shared."""

@@ -359,6 +359,22 @@ struct OnDevice {
   ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
 };
 
+static bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+static int capturing(kc_ctx* c, bool* is) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  CK(cudaStreamIsCapturing(c->stream, &st));
+  *is = st != cudaStreamCaptureStatusNone;
+  return KC_OK;
+}
+// A launch bracketed by the profile's events has no time of its own inside a graph.
+static int not_profiled_in_graph(kc_ctx* c, const char* where) {
+  bool is = false;
+  if (c->profile) RC(capturing(c, &is));
+  return is ? fail(KC_ERR_INVALID, "%s: captured while kc_profile_enable is on", where) : KC_OK;
+}
+
 extern "C" int kc_ctx_wait_stream(kc_ctx_t c, void* stream) {
   if (!c) return fail(KC_ERR_INVALID, "kc_ctx_wait_stream: ctx is NULL");
   if (stream == (void*)c->stream) return KC_OK;
@@ -787,14 +803,17 @@ extern "C" int kc_adapter_rows_create(kc_ctx_t c, const int32_t* slot_of_row, in
   }
   OnDevice on;
   CK(on.enter(c->device));
-  std::vector<int32_t> order(m);
-  for (int i = 0; i < m; ++i) order[i] = i;
-  std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return slot_of_row[a] < slot_of_row[b]; });
+  std::vector<int32_t> order;
   std::vector<LoraTile> tiles;
-  for (int i = 0, j; i < m; i = j) {
-    for (j = i; j < m && slot_of_row[order[j]] == slot_of_row[order[i]]; ++j) {}
-    for (int k = i; k < j; k += LORA_TILE) tiles.push_back(LoraTile{slot_of_row[order[i]], k, std::min(LORA_TILE, j - k)});
-  }
+  try {
+    order.resize(m);
+    for (int i = 0; i < m; ++i) order[i] = i;
+    std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return slot_of_row[a] < slot_of_row[b]; });
+    for (int i = 0, j; i < m; i = j) {
+      for (j = i; j < m && slot_of_row[order[j]] == slot_of_row[order[i]]; ++j) {}
+      for (int k = i; k < j; k += LORA_TILE) tiles.push_back(LoraTile{slot_of_row[order[i]], k, std::min(LORA_TILE, j - k)});
+    }
+  } catch (const std::bad_alloc&) { return fail(KC_ERR_OOM, "kc_adapter_rows_create: host memory"); }
   kc_adapter_rows* r = new kc_adapter_rows;
   r->ctx = c; r->device = c->device; r->m = m; r->n_tiles = (int)tiles.size(); r->max_slot = max_slot;
   const size_t t_bytes = tiles.size() * sizeof(LoraTile);
@@ -828,9 +847,13 @@ extern "C" int kc_adapters_apply(kc_adapters_t ad, kc_adapter_rows_t r, const vo
   if (ad->ctx != r->ctx) return fail(KC_ERR_INVALID, "kc_adapters_apply: adapters and rows belong to different contexts");
   if (r->max_slot >= ad->slots) return fail(KC_ERR_INVALID, "kc_adapters_apply: rows use slot %d of %d", r->max_slot, ad->slots);
   if ((uintptr_t)x_dev % 16 || (uintptr_t)y_dev % 2 || (uintptr_t)out_dev % 2) return fail(KC_ERR_INVALID, "kc_adapters_apply: x must be 16-byte aligned, y and out 2-byte");
+  const size_t x_bytes = (size_t)r->m * ad->n_in * sizeof(bf16), y_bytes = (size_t)r->m * ad->n_out * sizeof(bf16);
+  if (overlap(x_dev, x_bytes, out_dev, y_bytes)) return fail(KC_ERR_INVALID, "kc_adapters_apply: out overlaps x");
+  if (y_dev != out_dev && overlap(y_dev, y_bytes, out_dev, y_bytes)) return fail(KC_ERR_INVALID, "kc_adapters_apply: out overlaps y without being y");
   kc_ctx* c = ad->ctx;
   OnDevice on;
   CK(on.enter(ad->device));
+  RC(not_profiled_in_graph(c, "kc_adapters_apply"));
   LoraParams p{};
   p.x = (const bf16*)x_dev; p.y = (const bf16*)y_dev; p.out = (bf16*)out_dev;
   p.a = ad->a; p.b = ad->b; p.slots = ad->meta; p.tiles = r->tiles; p.rows = r->rows;
@@ -1802,12 +1825,13 @@ static_assert(sizeof(kc_sampling) == sizeof(DrawSetting) && alignof(DrawSetting)
 extern "C" int kc_sample_rows(kc_ctx_t c, const void* logits_dev, int64_t ld, int32_t rows, int32_t vocab, const kc_sampling* sampling_dev,
                               const float* uniform_dev, uint32_t* tokens_out_dev, float* logprobs_out_dev) {
   if (!c || !logits_dev || !sampling_dev || !uniform_dev || !tokens_out_dev) return fail(KC_ERR_INVALID, "kc_sample_rows: NULL argument");
-  if (rows < 1 || vocab < 1 || vocab > 1 << 30) return fail(KC_ERR_INVALID, "kc_sample_rows: [%d, %d]", rows, vocab);
+  if (rows < 1 || rows > 1 << 24 || vocab < 1 || vocab > 1 << 30) return fail(KC_ERR_INVALID, "kc_sample_rows: [%d, %d]", rows, vocab);
   if (ld < vocab && rows > 1) return fail(KC_ERR_INVALID, "kc_sample_rows: rows of %d values every %lld", vocab, (long long)ld);
   if ((uintptr_t)logits_dev % 2 || (uintptr_t)sampling_dev % 16 || (uintptr_t)uniform_dev % 4 || (uintptr_t)tokens_out_dev % 4 || (uintptr_t)logprobs_out_dev % 4)
     return fail(KC_ERR_INVALID, "kc_sample_rows: an argument is not aligned (logits 2 bytes, settings 16, the others 4)");
   OnDevice on;
   CK(on.enter(c->device));
+  RC(not_profiled_in_graph(c, "kc_sample_rows"));
   LAUNCH(c, KC_PROF_SAMPLE, 1, launch_draw_rows((const bf16*)logits_dev, ld, rows, vocab, reinterpret_cast<const DrawSetting*>(sampling_dev), uniform_dev,
                                                 tokens_out_dev, logprobs_out_dev, c->sm_count, c->stream));
   return KC_OK;
@@ -2085,18 +2109,54 @@ extern "C" int kc_paged_attention(kc_ctx_t c, kc_kv_t kv, int32_t layer, const v
   return rc;
 }
 
-// A step's attention kept as a handle: its metadata and workspace in a shell of its own, for softcap off and on (which kernel is the
-// faster one hangs on that).
+// A step's attention kept as a handle: plans for softcap off and on (which kernel is the faster one hangs on that), their metadata and
+// workspace in a shell. The second plan has a shell of its own only where its units are not the first one's.
 struct kc_attn_plan {
   kc_ctx* ctx = nullptr;
   kc_kv* kv = nullptr;
   int device = 0, num_heads = 0;
+  bool captured = false;   // a graph holds a run of it
   kc_model* shell[2] = {nullptr, nullptr};
+  bool apart = false;      // plan[1] lives in shell[1]
   StepPlan plan[2];
+  kc_model* shell_of(int capped) const { return shell[capped && apart ? 1 : 0]; }
 };
 static void free_attn_plan(kc_attn_plan* p) {
   for (kc_model* m : p->shell) if (m) free_model(m);
   delete p;
+}
+static bool same_units(const std::vector<AttnUnit>& a, const std::vector<AttnUnit>& b) {
+  return a.size() == b.size() && !memcmp(a.data(), b.data(), a.size() * sizeof(AttnUnit));
+}
+
+// Plans `seqs` into the handle. Buffers grow where they have to, so that a plan set step after step allocates nothing; the host waits
+// for the copies of two settings before at the most. Refused sequences leave the plan as it was; a failed copy or allocation
+// leaves it without one.
+static int set_attn_plan(kc_attn_plan* p, const kc_seq_step* seqs, int32_t n_seqs, const char* where) {
+  long long n = 0;
+  for (int i = 0; i < n_seqs; ++i) n += std::max(0, seqs[i].len);
+  if (n_seqs < 1 || n < 1 || n > 1 << 24) return fail(KC_ERR_INVALID, "%s: %lld token(s) of %d sequence(s)", where, n, n_seqs);
+  bool busy = false;
+  RC(capturing(p->ctx, &busy));
+  if (busy) return fail(KC_ERR_INVALID, "%s: the context's stream is being captured", where);
+  std::vector<uint32_t> ids((size_t)n, 0);
+  if (!p->shell[0]) RC(new_shell(p->ctx, &p->shell[0]));
+  set_shell(p->shell[0], p->kv, p->num_heads, (int)n, n_seqs);
+  StepPlan plan[2];
+  for (int capped = 0; capped < 2; ++capped)
+    RC(validate_step(p->shell[0], p->kv, ids.data(), (int32_t)n, seqs, n_seqs, 0, &plan[capped], true, capped != 0, false, true));
+  const bool apart = plan[0].shared.on != plan[1].shared.on || plan[0].whole != plan[1].whole || !same_units(plan[0].units, plan[1].units) ||
+                     !same_units(plan[0].shared.units, plan[1].shared.units);
+  if (apart && !p->shell[1]) RC(new_shell(p->ctx, &p->shell[1]));
+  if (apart) set_shell(p->shell[1], p->kv, p->num_heads, (int)n, n_seqs);
+  p->plan[0].n = p->plan[1].n = 0;
+  for (int i = 0; i < (apart ? 2 : 1); ++i) {
+    RC(upload_meta(p->shell[i], p->kv, ids.data(), seqs, plan[i]));
+    RC(ensure_attn_ws(p->shell[i], plan[i]));
+  }
+  p->apart = apart;
+  for (int i = 0; i < 2; ++i) p->plan[i] = std::move(plan[i]);
+  return KC_OK;
 }
 
 extern "C" int kc_attn_plan_create(kc_ctx_t c, kc_kv_t kv, const kc_seq_step* seqs, int32_t n_seqs, int32_t num_heads, kc_attn_plan_t* out) {
@@ -2104,30 +2164,32 @@ extern "C" int kc_attn_plan_create(kc_ctx_t c, kc_kv_t kv, const kc_seq_step* se
   if (kv->ctx != c) return fail(KC_ERR_INVALID, "kc_attn_plan_create: the pools belong to another context");
   if (num_heads < kv->kv_heads || num_heads % kv->kv_heads || num_heads / kv->kv_heads > 64)
     return fail(KC_ERR_INVALID, "kc_attn_plan_create: %d heads over %d kv heads", num_heads, kv->kv_heads);
-  long long n = 0;
-  for (int i = 0; i < n_seqs; ++i) n += std::max(0, seqs[i].len);
-  if (n_seqs < 1 || n < 1 || n > 1 << 24) return fail(KC_ERR_INVALID, "kc_attn_plan_create: %lld token(s) of %d sequence(s)", n, n_seqs);
   OnDevice on;
   CK(on.enter(c->device));
   kc_attn_plan* p = new kc_attn_plan;
   p->ctx = c; p->kv = kv; p->device = c->device; p->num_heads = num_heads;
-  std::vector<uint32_t> ids((size_t)n, 0);
-  int rc = KC_OK;
-  for (int capped = 0; capped < 2 && !rc; ++capped) {
-    kc_model* m = nullptr;
-    rc = new_shell(c, &m);
-    p->shell[capped] = m;
-    if (rc) break;
-    set_shell(m, kv, num_heads, (int)n, n_seqs);
-    rc = validate_step(m, kv, ids.data(), (int32_t)n, seqs, n_seqs, 0, &p->plan[capped], true, capped != 0, false, true);
-    if (!rc) rc = upload_meta(m, kv, ids.data(), seqs, p->plan[capped]);
-    if (!rc) rc = ensure_attn_ws(m, p->plan[capped]);
+  int rc;
+  try { rc = set_attn_plan(p, seqs, n_seqs, "kc_attn_plan_create"); }
+  catch (const std::bad_alloc&) { rc = fail(KC_ERR_OOM, "kc_attn_plan_create: host memory"); }
+  if (rc) {
+    std::string keep = g_err;
+    quiesce(c, c->device);
+    free_attn_plan(p);
+    g_err = keep;
+    return rc;
   }
-  if (!rc && cudaStreamSynchronize(c->stream) != cudaSuccess) rc = fail(KC_ERR_CUDA, "kc_attn_plan_create: the copy of the plan failed");
-  if (rc) { std::string keep = g_err; free_attn_plan(p); g_err = keep; return rc; }
   g_live++;
   *out = p;
   return KC_OK;
+}
+
+extern "C" int kc_attn_plan_set(kc_attn_plan_t p, const kc_seq_step* seqs, int32_t n_seqs) {
+  if (!p || !seqs) return fail(KC_ERR_INVALID, "kc_attn_plan_set: NULL argument");
+  if (p->captured) return fail(KC_ERR_INVALID, "kc_attn_plan_set: a graph was captured over this plan; it needs the plan as it is");
+  OnDevice on;
+  CK(on.enter(p->device));
+  try { return set_attn_plan(p, seqs, n_seqs, "kc_attn_plan_set"); }
+  catch (const std::bad_alloc&) { return fail(KC_ERR_OOM, "kc_attn_plan_set: host memory"); }
 }
 
 extern "C" int kc_attn_plan_keys(kc_attn_plan_t p, int64_t* read, int64_t* apart) {
@@ -2154,11 +2216,18 @@ extern "C" int kc_attn_plan_run(kc_attn_plan_t p, int32_t layer, const void* q_d
   if (!p || !q_dev || !out_dev) return fail(KC_ERR_INVALID, "kc_attn_plan_run: NULL argument");
   if (layer < 0 || layer >= p->kv->layers) return fail(KC_ERR_INVALID, "kc_attn_plan_run: layer %d of %d", layer, p->kv->layers);
   if ((uintptr_t)q_dev % 16 || (uintptr_t)out_dev % 16) return fail(KC_ERR_INVALID, "kc_attn_plan_run: q and out must be 16-byte aligned");
+  const int capped = softcap > 0.f ? 1 : 0;
+  kc_model* m = p->shell_of(capped);
+  const StepPlan& plan = p->plan[capped];
+  if (plan.n == 0) return fail(KC_ERR_INVALID, "kc_attn_plan_run: the plan was not set");
+  const size_t bytes = (size_t)plan.n * p->num_heads * p->kv->head_dim * sizeof(bf16);
+  if (overlap(q_dev, bytes, out_dev, bytes)) return fail(KC_ERR_INVALID, "kc_attn_plan_run: out overlaps q");
   OnDevice on;
   CK(on.enter(p->device));
-  const int capped = softcap > 0.f ? 1 : 0;
-  kc_model* m = p->shell[capped];
-  const StepPlan& plan = p->plan[capped];
+  bool in_graph = false;
+  RC(capturing(p->ctx, &in_graph));
+  RC(not_profiled_in_graph(p->ctx, "kc_attn_plan_run"));
+  p->captured |= in_graph;
   RC(ensure_q_maps(m, (const bf16*)q_dev, plan.n, p->num_heads, p->num_heads / p->kv->kv_heads, plan));
   return run_attention(m, p->kv, plan, layer, (bf16*)out_dev, scale, softcap, window, p->num_heads, true);
 }

@@ -199,6 +199,42 @@ def test_windows_layers_streams_and_graphs(ctx):
     assert ctx.device_status() == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (16, 8, 256)])
+def test_a_plan_is_set_step_after_step(ctx, heads, kv_heads, dim):
+    """One plan for steps that follow one another without a wait: more rows and fewer, with what is shared and without, capped
+    (which may want other units) and not. Every step has paged_attention's bits. A graph ends the setting."""
+    seqs, total = tables([(2048, [(4, 2100 + 20 * i) for i in range(50)]), (0, [(1, 300), (40, 0)])], 16, 1)
+    kv, _ = pools(ctx, kv_heads, dim, total, 16, 4)
+    steps = [[api.SeqStep(n, s.offset + at, 0, s.blocks) for s in seqs[:50]] for at, n in ((0, 1), (1, 1), (2, 2))]
+    steps += [seqs[50:], seqs, seqs[3:4], steps[0]]
+    q = torch.randn(sum(s.len for s in seqs), heads, dim, device="cuda").to(torch.bfloat16)
+    plan, got, sharing = api.AttentionPlan(ctx, kv, heads, seqs[50:51]), [], []
+    torch.cuda.synchronize()
+    for step in steps:
+        plan.set(step)
+        assert plan.tokens == sum(s.len for s in step)
+        sharing.append(shares(plan))
+        got.append([plan.run(0, q[: plan.tokens], dim ** -0.5, cap) for cap in (0.0, 20.0)])
+    with pytest.raises(api.KcError):
+        plan.set([api.SeqStep(1, -1, 0, seqs[0].blocks)])
+    assert plan.tokens == 50
+    got.append([plan.run(0, q[:50], dim ** -0.5, cap) for cap in (0.0, 20.0)])
+    torch.cuda.synchronize()
+    assert sharing == [True, True, True, False, False, False, True]     # a step with 40 rows of a prompt keeps to the sequences' own units
+    for step, outs in zip(steps + steps[:1], got):
+        n = sum(s.len for s in step)
+        for out, cap in zip(outs, (0.0, 20.0)):
+            assert torch.equal(out, api.paged_attention(ctx, kv, 0, q[:n], step, dim ** -0.5, cap))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = plan.run(0, q[:50], dim ** -0.5)
+    with pytest.raises(api.KcError):
+        plan.set(steps[1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, got[0][0])
+
+
 def test_large_scores(ctx):
     """One key outweighs all others by far: maxima that move by thousands of binary orders from chunk to chunk."""
     seqs, total = tables([(2048, [(1, 2060 + 9 * i) for i in range(80)])], 16, 1)

@@ -1,0 +1,155 @@
+"""What the entry points that are queued without waiting refuse, and what their handles ask of the CUDA runtime, against a
+stand-in for it. Needs no GPU; each test is a process of its own."""
+import subprocess
+
+import pytest
+
+from tests.test_host_calls import ROOT, fake, run  # noqa: F401  (a fixture)
+
+
+@pytest.fixture(scope="module")
+def graphs(fake, tmp_path_factory):  # noqa: F811
+    so = tmp_path_factory.mktemp("fake") / "fake_cudart_graphs.so"
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-I/usr/local/cuda/include", "-o", str(so), str(ROOT / "tests" / "fake_cudart_graphs.cpp")], check=True)
+    return f"{fake}:{so}"
+
+
+PLAN = """
+def steps(lens, n_blocks=None, blocks=table):
+    return (L.KcSeqStep * max(1, len(lens)))(*[L.KcSeqStep(n, off, 0, -(-(n + off) // 16) if n_blocks is None else n_blocks, blocks) for n, off in lens])
+def create(lens, heads=4, **kw):
+    p = C.c_void_p()
+    return lib.kc_attn_plan_create(ctx, kv, steps(lens, **kw), len(lens), heads, C.byref(p)), p
+def launches():
+    return [c for c in calls() if c.startswith("launch")]
+"""
+
+
+def test_plans_are_refused(graphs):
+    run(graphs, PLAN + """
+before = lib.kc_live_objects()
+far = (C.c_uint32 * 80)(*range(1, 81))
+for bad in (dict(lens=[]), dict(lens=[(0, 5)]), dict(lens=[(1, 5), (0, 5)]), dict(lens=[(-1, 5)]), dict(lens=[(1, -1)]), dict(lens=[(1, 5)], heads=3), dict(lens=[(1, 5)], heads=0),
+            dict(lens=[(1, 5)], heads=130), dict(lens=[(1, 40)], n_blocks=2), dict(lens=[(1, 1272)], blocks=far), dict(lens=[(1, 5)], blocks=None), dict(lens=[((1 << 24) + 1, 0)])):
+    rc, p = create(**bad)
+    assert rc == L.KC_ERR_INVALID and not p.value and lib.kc_last_error(), bad
+for a in ((None, kv, steps([(1, 5)])), (ctx, None, steps([(1, 5)])), (ctx, kv, None)):
+    assert lib.kc_attn_plan_create(*a, 1, 4, C.byref(C.c_void_p())) == L.KC_ERR_INVALID
+assert lib.kc_attn_plan_create(ctx, kv, steps([(1, 5)]), 1, 4, None) == L.KC_ERR_INVALID
+fake.fake_capture(1)
+assert create([(1, 5)])[0] == L.KC_ERR_INVALID     # its copies are not part of a graph
+fake.fake_capture(0)
+assert lib.kc_live_objects() == before
+rc, p = create([(3, 40), (1, 0)])
+ok(rc)
+def attend(plan=p, layer=0, q=at, out=at + 4 * 4 * 64 * 2):
+    return lib.kc_attn_plan_run(plan, layer, q, 0.125, 0.0, 0, out)
+fake.fake_reset()
+for bad in (dict(plan=None), dict(layer=-1), dict(layer=1), dict(q=None), dict(q=at + 8), dict(out=None), dict(out=at + 4 * 4 * 64 * 2 + 2), dict(out=at), dict(out=at + 4 * 4 * 64 * 2 - 16), dict(q=at + 16, out=at)):
+    assert attend(**bad) == L.KC_ERR_INVALID, bad
+assert lib.kc_attn_plan_keys(None, C.byref(C.c_int64()), C.byref(C.c_int64())) == L.KC_ERR_INVALID
+assert lib.kc_attn_plan_set(None, steps([(1, 5)]), 1) == L.KC_ERR_INVALID and lib.kc_attn_plan_set(p, None, 1) == L.KC_ERR_INVALID
+assert not launches()
+ok(attend())
+assert launches()
+lib.kc_attn_plan_free(p)
+lib.kc_attn_plan_free(None)
+assert lib.kc_live_objects() == before
+""")
+
+
+def test_a_plan_is_set_again(graphs):
+    """No allocation while the plan has room, one copy a setting, no wait of the host; a refused step leaves the plan as it was."""
+    run(graphs, PLAN + """
+rc, p = create([(3, 40), (1, 0)])
+ok(rc)
+read, apart = C.c_int64(), C.c_int64()
+def keys():
+    ok(lib.kc_attn_plan_keys(p, C.byref(read), C.byref(apart)))
+    return apart.value
+assert keys() == 43 + 1
+fake.fake_reset()
+for off in range(41, 50):
+    ok(lib.kc_attn_plan_set(p, steps([(3, off)]), 1))
+    assert keys() == off + 3
+assert calls() == ["copy"] * 9
+assert lib.kc_attn_plan_set(p, steps([(3, -1)]), 1) == L.KC_ERR_INVALID and lib.kc_attn_plan_set(p, steps([]), 0) == L.KC_ERR_INVALID
+assert keys() == 52 and not calls()
+q, out = at, at + (1 << 19)
+ok(lib.kc_attn_plan_run(p, 0, q, 0.125, 0.0, 0, out))
+fake.fake_fail_above(1 << 16)                      # a step that the plan has no room for, and no memory for it
+assert lib.kc_attn_plan_set(p, steps([(1, 1200)] * 600), 600) == L.KC_ERR_OOM
+assert lib.kc_attn_plan_run(p, 0, q, 0.125, 0.0, 0, out) == L.KC_ERR_INVALID
+fake.fake_fail_above(2 ** 62)
+ok(lib.kc_attn_plan_set(p, steps([(1, 1200)] * 60), 60))
+ok(lib.kc_attn_plan_run(p, 0, q, 0.125, 0.0, 0, out))
+fake.fake_capture(1)
+assert lib.kc_attn_plan_set(p, steps([(1, 5)]), 1) == L.KC_ERR_INVALID
+ok(lib.kc_attn_plan_run(p, 0, q, 0.125, 0.0, 0, out))
+fake.fake_capture(0)
+assert lib.kc_attn_plan_set(p, steps([(1, 5)]), 1) == L.KC_ERR_INVALID     # the graph needs the plan as it is
+assert b"graph" in lib.kc_last_error()
+ok(lib.kc_attn_plan_run(p, 0, q, 0.125, 0.0, 0, out))
+lib.kc_attn_plan_free(p)
+""")
+
+
+def test_no_times_from_a_graph(graphs):
+    """The profile's events have no time inside a graph: a capture while it is on is refused, behind it all is as ever."""
+    run(graphs, PLAN + """
+rc, p = create([(3, 40)])
+ok(rc)
+ok(lib.kc_profile_enable(ctx, 1))
+def both():
+    return {lib.kc_attn_plan_run(p, 0, at, 0.125, 0.0, 0, at + 4096), lib.kc_sample_rows(ctx, at, 100, 2, 100, at, at, at, None)}
+assert both() == {L.KC_OK}
+fake.fake_capture(1)
+assert both() == {L.KC_ERR_INVALID}
+ok(lib.kc_profile_enable(ctx, 0))
+assert both() == {L.KC_OK}
+""")
+
+
+def test_adapters_are_refused(graphs):
+    run(graphs, """
+before = lib.kc_live_objects()
+def create(n_in=64, n_out=48, slots=3, rank=20):
+    p = C.c_void_p()
+    return lib.kc_adapters_create(ctx, n_in, n_out, slots, rank, C.byref(p)), p
+for bad in (dict(n_in=0), dict(n_in=-32), dict(n_in=48), dict(n_out=0), dict(slots=0), dict(slots=(1 << 20) + 1), dict(rank=0), dict(rank=-1)):
+    assert create(**bad)[0] == L.KC_ERR_INVALID, bad
+assert create(rank=129)[0] == L.KC_ERR_UNSUPPORTED
+fake.fake_fail_above(1 << 12)
+assert create()[0] == L.KC_ERR_OOM
+fake.fake_fail_above(2 ** 62)
+assert lib.kc_live_objects() == before
+rc, bank = create()
+ok(rc)
+for a in ((-1, at, at, 4, 1.0), (3, at, at, 4, 1.0), (0, None, at, 4, 1.0), (0, at, None, 4, 1.0), (0, at, at, 21, 1.0), (0, at, at, -1, 1.0), (0, at, at, 4, float("nan")), (0, at, at, 4, float("inf"))):
+    assert lib.kc_adapters_set(bank, *a, 0) == L.KC_ERR_INVALID, a
+assert lib.kc_adapters_set(None, 0, at, at, 4, 1.0, 0) == L.KC_ERR_INVALID
+ok(lib.kc_adapters_set(bank, 2, at, at, 20, 1.0, 0)); ok(lib.kc_adapters_set(bank, 2, None, None, 0, 0.0, 0))
+def rows(*slots, m=None):
+    p = C.c_void_p()
+    return lib.kc_adapter_rows_create(ctx, (C.c_int32 * max(1, len(slots)))(*slots), len(slots) if m is None else m, C.byref(p)), p
+for bad in (rows(), rows(0, m=-1), rows(0, m=(1 << 24) + 1), rows(0, -2)):
+    assert bad[0] == L.KC_ERR_INVALID
+rc, who = rows(2, -1, 0, 2)
+ok(rc)
+rc, past = rows(0, 3)
+ok(rc)
+out = at + (1 << 16)
+def apply(bank=bank, who=who, x=at, y=out, out=out):
+    return lib.kc_adapters_apply(bank, who, x, y, out)
+fake.fake_reset()
+x_bytes, y_bytes = 4 * 64 * 2, 4 * 48 * 2
+for bad in (dict(bank=None), dict(who=None), dict(x=None), dict(y=None), dict(out=None), dict(who=past), dict(x=at + 2), dict(y=out + 1), dict(out=out + 1), dict(out=at), dict(out=at + x_bytes - 2),
+            dict(x=at + 256, out=at + 256 - y_bytes + 2), dict(y=out + 2), dict(y=out + y_bytes - 2), dict(y=out - y_bytes + 2)):
+    assert apply(**bad) == L.KC_ERR_INVALID, bad
+assert not calls()
+ok(apply()); ok(apply(y=out + y_bytes)); ok(apply(x=at, out=at + x_bytes)); ok(apply(y=out + 1024 + 2, out=out + 2))
+assert len([c for c in calls() if c.startswith("launch")]) == 4
+for h in (past, who): lib.kc_adapter_rows_free(h)
+lib.kc_adapters_free(bank); lib.kc_adapters_free(None); lib.kc_adapter_rows_free(None)
+assert lib.kc_live_objects() == before
+""")
