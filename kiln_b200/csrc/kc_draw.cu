@@ -12,9 +12,16 @@
 // summed in a fixed tree over the values, whatever the number of CTAs a row has.
 //
 // Counting: a bin a value, of the magnitudes [2^-24, 2^8) of either sign (the home window), 32 KB of shared memory. A row with
-// other magnitudes takes another pass over itself for each of the eight other windows of 32 binary orders that it has values in, so that
-// any row is exact; zeros are counted apart. The counts and masses of the binades lie in shared memory of every CTA of the row's
-// cluster, which then all look for the same borders.
+// other magnitudes (but for -inf) takes another pass over itself for each of the eight other windows of 32 binary orders that it has values
+// in, so that any row is exact; zeros are counted apart. The counts and masses of the binades lie in shared memory of every CTA of the row's
+// cluster, which then all look for the same borders. A bin also adds up where its values stand, so that a value that a CTA has once
+// is found without another pass: 512 rows of 256000 159 -> 141 us.
+//
+// What bounds it. Few rows: launch, three cluster barriers and the search's chains of latencies, 2200 cycles a border: one row of 128256 11.6 us,
+// seven of 50001 13.0. Many: the counting, at 0.7 of what shared memory's atomics take (3.6 wavefronts for a warp's 32 places: half of a
+// CTA's 37000 cycles at 64128 values), and behind it the accounts and the search, which only the SM's other CTA can fill: 128 rows
+// of 128256 31 us, 192 41 (384 CTAs in 296 places, 7.5 us at a copy's rate), 512 of 256000 140 (40). Three CTAs an SM of 256 to 384 threads:
+// 40 to 44 and 153 to 162; one CTA a row 47 at 192.
 #include "kc_fused.cuh"
 #include "kc_umma.cuh"
 
@@ -22,12 +29,16 @@ namespace kc {
 
 namespace {
 
-constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32;
+// Threads of a CTA: half as many where a row has many CTAs, whose barriers then take less (one row of 128256 12.8 -> 11.5 us; with two CTAs a row
+// 512 rows of 256000 141 -> 159 us).
+constexpr int draw_threads(int ctas) { return ctas > 2 ? 256 : 512; }
 constexpr int DRAW_WINDOW = 4096;                 // magnitudes (bf16 without the sign) of a window, 32 binades
 constexpr int DRAW_LOW = 4, DRAW_SIDE = 4128;     // of a sign's bins: the window's first one; all of them (next to the window's: what lies below, above)
 constexpr int DRAW_HOME = 4;                      // the window that holds a language model's logits: magnitudes 2^-24 to 2^8
 constexpr int DRAW_BASE0 = 103 * 128 - DRAW_HOME * DRAW_WINDOW;   // first magnitude of window 0 (below zero: it is a short one)
 constexpr int DRAW_WINDOWS = 9;
+// A bin counts in its low bits and adds up the indices of the vectors in the high ones, which is the place of a value that occurs once.
+constexpr int DRAW_AT = 18;
 // Binades in falling order of value: a run of 32 for each window, the positive ones' from the last window to the first, a run
 // that holds zero alone, the negative ones'.
 constexpr int DRAW_ZERO = DRAW_WINDOWS, DRAW_RUNS = 2 * DRAW_WINDOWS + 1;
@@ -37,18 +48,20 @@ static_assert(DRAW_BASE0 % 128 == 0 && DRAW_BASE0 + DRAW_WINDOWS * DRAW_WINDOW >
 // C: CTAs of a row's cluster. Every C-th binade of the resident window is a CTA's own, to add up over the cluster's parts of the row.
 template <int C>
 struct DrawShared {
-  uint32_t bins[2 * DRAW_SIDE];                   // [sign][magnitude]: how often the value occurs in this CTA's part of the row
+  uint32_t bins[2 * DRAW_SIDE];                   // [sign][magnitude]: how often the value occurs in this CTA's part of the row, and where (DRAW_AT)
   double lane_weight[64 / C][32];                 // own binades, four values a lane: the weight of the lane's first one,
   double lane_mass[64 / C][32];                   // mass and
   uint32_t lane_count[64 / C][32];                // tokens of the binade up to the lane's last one
+  uint4 lane_counts[64 / C][32];                  // how often each value occurs in the row, in falling order
   double mass[DRAW_RUNS][32];                     // of a binade; later of its run up to it
   uint32_t count[DRAW_RUNS][32];
   uint32_t peer_top[8], peer_seen[8], peer_zeros[8], peer_match[8];   // what each CTA of the cluster found
-  uint32_t warp_a[DRAW_WARPS], warp_b[DRAW_WARPS];
+  uint32_t warp_a[draw_threads(C) / 32], warp_b[draw_threads(C) / 32];
+  uint32_t far;                                   // whether a finite value lies below the window's negative ones
   uint32_t above;                                 // tokens of w >= min_p, over the cluster
   double ratio[32];                               // of the weights of neighbouring values, by binade of the resident window
   int window;                                     // the one that the search wants resident; -1: it is done
-  uint32_t bits, taken, times; double weight, mass_kept;   // its result
+  uint32_t bits, taken; double weight, mass_kept;   // its result
 };
 
 __device__ __forceinline__ void peer_put(uint32_t* p, uint32_t rank, uint32_t v) {
@@ -148,10 +161,11 @@ struct DrawRow {
 };
 
 template <int C>
-__global__ void __launch_bounds__(DRAW_THREADS, 2)
+__global__ void __launch_bounds__(draw_threads(C), 2)
 draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const DrawSetting* __restrict__ settings,
                  const float* __restrict__ uniform, uint32_t* __restrict__ tokens, float* __restrict__ logprobs,
                  uint32_t* __restrict__ tokens_host, float* __restrict__ logprobs_host, int skip_greedy) {
+  constexpr int DRAW_THREADS = draw_threads(C), DRAW_WARPS = DRAW_THREADS / 32;
   extern __shared__ __align__(16) uint8_t draw_smem[];
   DrawShared<C>& s = *reinterpret_cast<DrawShared<C>*>(draw_smem);
   pdl_launch_dependents();
@@ -163,7 +177,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
   };
   clear_bins();
   for (int i = tid; i < DRAW_RUNS * 32; i += DRAW_THREADS) { s.mass[0][i] = 0.0; s.count[0][i] = 0; }
-  if (tid == 0) s.above = 0;
+  if (tid == 0) s.above = s.far = 0;
   __syncthreads();                       // the bins are clear before any thread counts: the arrival above says nothing about them
   cluster_wait();
   pdl_wait();
@@ -182,25 +196,29 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
   const DrawRow x(logits + (size_t)row_index * ld, vocab);
   const int vecs = x.vecs(), per = (vecs + C - 1) / C;
   const int v0 = min(vecs, rank * per), v1 = skip ? v0 : min(vecs, v0 + per);
+  const bool places_fit = per <= 1 << (32 - DRAW_AT);   // 8 values a vector: their counts fit below then too
+  const uint32_t at_step = places_fit ? 1u << DRAW_AT : 0u, count_mask = places_fit ? (1u << DRAW_AT) - 1 : ~0u;
+  static_assert(8 << (32 - DRAW_AT) < 1 << DRAW_AT, "counts");
 
   // ---- pass over the row: bins of the home window, and the maximum. Two values at a time as halves of a register: their
   // magnitudes, held between the window's neighbours on either side, become places of bins by whole-number arithmetic that
   // neither half carries out of ----
-  uint32_t top = 0xFF80FF80u;
+  uint32_t top = 0xFF80FF80u, far = 0;   // far: of -inf 0, of a finite negative value its bits and 0x80: largest where the magnitude is
   constexpr uint32_t FIRST = DRAW_BASE0 + DRAW_HOME * DRAW_WINDOW;
   uint8_t* const bin_bytes = reinterpret_cast<uint8_t*>(s.bins);
   if (greedy) {
     x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int) { top = top_bf162(top, top_bf162(top_bf162(u.x, u.y), top_bf162(u.z, u.w))); });
   } else {
-    x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int) {
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int v) {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w}, one = 1u + (uint32_t)(v - v0) * at_step;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         top = top_bf162(top, w[j]);
+        far = __viaddmax_u16x2(w[j], 0x00800080u, far);
         const uint32_t mag = low_bf162(top_bf162(w[j] & 0x7FFF7FFFu, (FIRST - 1) * 0x10001u), (FIRST + DRAW_WINDOW) * 0x10001u);
         const uint32_t at = mag * 4 + ((w[j] >> 15) & 0x00010001u) * (DRAW_SIDE * 4) - (FIRST - DRAW_LOW) * 4 * 0x10001u;   // bytes: 32912 at the most
-        atomicAdd(reinterpret_cast<uint32_t*>(bin_bytes + (at & 0xFFFFu)), 1u);
-        atomicAdd(reinterpret_cast<uint32_t*>(bin_bytes + (at >> 16)), 1u);
+        atomicAdd(reinterpret_cast<uint32_t*>(bin_bytes + (at & 0xFFFFu)), one);
+        atomicAdd(reinterpret_cast<uint32_t*>(bin_bytes + (at >> 16)), one);
       }
     });
   }
@@ -208,13 +226,15 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
     const float2 two = unpack_bf162(top);
     const float m = warp_max(fmaxf(two.x, two.y));
     if (lane == 0) s.warp_a[warp] = __float_as_uint(m);
+    constexpr uint32_t FAR = 0x8000u + FIRST + DRAW_WINDOW + 0x80u;
+    if ((far & 0xFFFFu) >= FAR || (far >> 16) >= FAR) s.far = 1;
   }
   __syncthreads();
   const float m_cta = warp_max(__uint_as_float(s.warp_a[lane & (DRAW_WARPS - 1)]));
-  // Values outside the home window (masked ones and NaN among them): zeros are counted, of the others what windows they are in.
+  // Values outside the home window (NaN among them, masked ones not): zeros are counted, of the others what windows they are in.
   uint32_t seen = 0, zeros = 0;
   constexpr int HIGH = DRAW_LOW + DRAW_WINDOW;
-  if (!greedy && (s.bins[DRAW_LOW - 1] | s.bins[HIGH] | s.bins[DRAW_SIDE + DRAW_LOW - 1] | s.bins[DRAW_SIDE + HIGH])) {
+  if (!greedy && (s.bins[DRAW_LOW - 1] | s.bins[HIGH] | s.bins[DRAW_SIDE + DRAW_LOW - 1] | s.far)) {
     x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int) {
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -246,8 +266,8 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
   largest += 0.f;                        // -0 is +0
   // From here on every branch that holds a barrier is taken by the whole cluster: what it hangs on is the same in all its CTAs.
   const bool empty = largest == -INFINITY;   // nothing but masked tokens and NaN: token 0
-  uint32_t bits = __float_as_uint(largest) >> 16, taken = 1, times = 0;   // times: how often the value occurs, 0: not known
-  float logprob = empty ? -INFINITY : 0.f;
+  uint32_t bits = __float_as_uint(largest) >> 16, taken = 1;
+  int resident = DRAW_HOME;              // window of the bins
 
   if (!greedy && !empty) {
     const double top_value = largest, min_p = set.min_p;
@@ -255,7 +275,6 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
       const float l = value_of(b);
       return l == largest ? 1.0 : largest == INFINITY ? 0.0 : exp(((double)l - top_value) * inv_t);
     };
-    int resident = DRAW_HOME;
     // A binade's 128 values are four a lane, in falling order: of the k-th binade of the resident window (negative ones from 32 on) the place of
     // this lane's bins, and whether they lie in falling order of value as they are.
     auto place = [&](int k, int of_lane) { return (k >> 5) * DRAW_SIDE + DRAW_LOW + (k & 31) * 128 + 4 * ((k >> 5) ? of_lane : 31 - of_lane); };
@@ -278,17 +297,20 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
         if (c[i]) w[i] = chained && value_of(b + i * d) != largest ? first : weight_of(b + i * d);
       }
     };
+    // The cluster's counts of this lane's values.
+    auto counts = [&](int k) {
+      uint4 o[C], v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < C; ++r) o[r] = peer_get4(&s.bins[place(k, lane)], (rank + r) & (C - 1));
+#pragma unroll
+      for (int r = 0; r < C; ++r) { v.x += o[r].x & count_mask; v.y += o[r].y & count_mask; v.z += o[r].z & count_mask; v.w += o[r].w & count_mask; }
+      return v;
+    };
     // Adds the cluster's bins of the resident window and what lanes hold of each binade; `enters`: its totals into every CTA's.
     auto account = [&](bool enters) {
-      for (int k = rank + C * warp; k < 64; k += C * DRAW_WARPS) {
-        uint4* own = reinterpret_cast<uint4*>(&s.bins[place(k, lane)]);
-        uint4 v = *own;
-#pragma unroll
-        for (int r = 1; r < C; ++r) {
-          const uint4 o = peer_get4(&s.bins[place(k, lane)], (rank + r) & (C - 1));
-          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
-        *own = v;                        // no other CTA reads these bins of this one before the next barrier
+      for (int i = rank + C * warp; i < 64; i += C * DRAW_WARPS) {
+        const int k = i < 32 ? i : 32 + ((i + 16) & 31);   // a row's values lie in the same ten or so binades of either sign: one of them a warp
+        uint4 v = counts(k);
         if (!__any_sync(0xffffffffu, (v.x | v.y | v.z | v.w) != 0)) continue;
         v = in_order(k, v);
         const uint32_t c[4] = {v.x, v.y, v.z, v.w};
@@ -308,7 +330,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
           const double mu = __shfl_up_sync(0xffffffffu, m, o);
           if (lane >= o) { n += nu; m += mu; }
         }
-        s.lane_weight[k / C][lane] = first; s.lane_mass[k / C][lane] = m; s.lane_count[k / C][lane] = n;
+        s.lane_counts[k / C][lane] = v; s.lane_weight[k / C][lane] = first; s.lane_mass[k / C][lane] = m; s.lane_count[k / C][lane] = n;
         if (!enters) continue;
         above = __reduce_add_sync(0xffffffffu, above);
         n = __shfl_sync(0xffffffffu, n, 31); m = __shfl_sync(0xffffffffu, m, 31);
@@ -327,12 +349,12 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
       __syncthreads();
       resident = window;
       const uint32_t base = DRAW_BASE0 + window * DRAW_WINDOW;
-      x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int v) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w}, one = 1u + (uint32_t)(v - v0) * at_step;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t b = (w[j >> 1] >> (16 * (j & 1))) & 0xFFFFu, mag = b & 0x7FFFu;
-          if (mag - base < DRAW_WINDOW && mag != 0 && (mag < BF16_INF || b == BF16_INF)) atomicAdd(&s.bins[(b >> 15) * DRAW_SIDE + DRAW_LOW + mag - base], 1u);
+          if (mag - base < DRAW_WINDOW && mag != 0 && (mag < BF16_INF || b == BF16_INF)) atomicAdd(&s.bins[(b >> 15) * DRAW_SIDE + DRAW_LOW + mag - base], one);
         }
       });
       cluster_sync();
@@ -376,7 +398,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
       }
       n = __shfl_sync(0xffffffffu, n_run, 31); mass = __shfl_sync(0xffffffffu, m_run, 31);
     }
-    struct { uint32_t bits, taken, times, n; double mass, weight; } at = {0, 0, 0, 0, 0.0, 0.0};   // value, how many of it out of how many, ..
+    struct { uint32_t bits, taken, n; double mass, weight; } at = {0, 0, 0, 0.0, 0.0};   // value, how many of it, tokens and mass up to there
     auto crossed = [](int what, uint32_t count, double m, uint32_t want, double target) { return what == COUNT ? count >= want : what == REACH ? m >= target : m > target; };
     // The border that a number of tokens (COUNT) or a mass reaches (REACH) or exceeds (EXCEED): in `at` with -1 returned, or
     // the window that has to be resident; -2 where nothing reaches it. Run, binade, lane, value: of each the first one at whose
@@ -408,7 +430,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
         ln = peer_get(&s.lane_count[k / C][lane], owner);
         lm = peer_get(&s.lane_mass[k / C][lane], owner);
         const double lw = peer_get(&s.lane_weight[k / C][lane], owner);
-        const uint4 v = in_order(k, peer_get4(&s.bins[place(k, lane)], owner));
+        const uint4 v = peer_get4(&s.lane_counts[k / C][lane].x, owner);
         const int who = first_of((v.x | v.y | v.z | v.w) && crossed(what, cn + ln, cm + lm, want, target), (v.x | v.y | v.z | v.w) != 0);
         cn += ahead_of(ln, who); cm += mass_ahead_of(lm, who);
         c[0] = __shfl_sync(0xffffffffu, v.x, who); c[1] = __shfl_sync(0xffffffffu, v.y, who);
@@ -437,7 +459,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
         while (r > 1 && crossed(what, 0, cm + (r - 1) * w_at, 0, target)) --r;
         while (r < c_at && !crossed(what, 0, cm + r * w_at, 0, target)) ++r;
       }
-      at.bits = b + i_at * d; at.taken = r; at.times = c_at; at.n = cn + r; at.mass = cm + r * w_at; at.weight = w_at;
+      at.bits = b + i_at * d; at.taken = r; at.n = cn + r; at.mass = cm + r * w_at; at.weight = w_at;
       return -1;
     };
     const double unit = u01 < 0.f ? 0.0 : (double)u01;
@@ -470,7 +492,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
         }
         if (lane == 0) {
           s.window = window < 0 ? -1 : window;
-          s.bits = at.bits; s.taken = at.taken; s.times = at.times; s.weight = at.weight; s.mass_kept = mass;
+          s.bits = at.bits; s.taken = at.taken; s.weight = at.weight; s.mass_kept = mass;
         }
       }
       __syncthreads();
@@ -478,12 +500,12 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
       enter(s.window, false);
       cluster_sync();
     }
-    bits = s.bits; taken = s.taken; times = s.times;
-    logprob = (float)log(s.weight / s.mass_kept);
+    bits = s.bits; taken = s.taken;
   }
 
   // ---- the token: occurrence `taken` of the value, in order of index ----
   auto write = [&](uint32_t token) {
+    const float logprob = empty ? -INFINITY : greedy ? 0.f : (float)log(s.weight / s.mass_kept);
     tokens[row_index] = token;
     if (logprobs) logprobs[row_index] = logprob;
     if (tokens_host) tokens_host[row_index] = token;
@@ -500,33 +522,45 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
     for (int j = 0; j < 4; ++j) mask |= (m[j] & 1u) << (2 * j) | (m[j] >> 31) << (2 * j + 1);
     return mask;
   };
-  if (times == 1 && !empty) {            // wherever it is
+  // A drawn value's bins say which CTA has the occurrence, and where, if that CTA has no other one.
+  const uint32_t place = (bits & 0x7FFFu) - (uint32_t)(DRAW_BASE0 + resident * DRAW_WINDOW);
+  const bool binned = !greedy && !empty && bits != 0 && place < DRAW_WINDOW;
+  uint32_t ahead = 0, mine = 0, m[4];
+  if (binned) {
+    const uint32_t* bin = &s.bins[(bits >> 15) * DRAW_SIDE + DRAW_LOW + place];
+    const uint32_t own = *bin & count_mask;
+    ahead = __reduce_add_sync(0xffffffffu, lane < rank ? peer_get(bin, lane) & count_mask : 0u);
     cluster_arrive();
-    uint32_t m[4];
-    x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int v) { if (matches(u, m)) write((uint32_t)(8 * v - x.shift + __ffs(places(m)) - 1)); });
-    cluster_wait();                      // the last access to another CTA's shared memory lies ahead of its arrival
-    return;
+    const bool here = taken > ahead && taken <= ahead + own, known = own == 1 && places_fit;
+    if (here && known && tid == 0) {
+      const int v = v0 + (int)(*bin >> DRAW_AT);
+      matches(x.vec(v), m);
+      write((uint32_t)(8 * v - x.shift + __ffs(places(m)) - 1));
+    }
+    if (!here || known) { cluster_wait(); return; }   // the last access to another CTA's shared memory lies ahead of its arrival
   }
   const int each = ((v1 - v0) + DRAW_WARPS - 1) / DRAW_WARPS;   // vectors of a warp, one after the other
   const int w0 = min(v1, v0 + warp * each), w1 = min(v1, w0 + each);
-  uint32_t mine = 0, m[4];
   if (!empty) x.each<32>(w0, w1, lane, [&](const uint4& u, int) { if (matches(u, m)) mine += __popc(places(m)); });
   mine = __reduce_add_sync(0xffffffffu, mine);
   if (lane == 0) s.warp_a[warp] = mine;
   __syncthreads();
-  if (tid < C) {
-    uint32_t all = 0;
-    for (int w = 0; w < DRAW_WARPS; ++w) all += s.warp_a[w];
-    peer_put(&s.peer_match[rank], tid, all);
+  if (binned) {
+    cluster_wait();
+  } else {
+    if (tid < C) {
+      uint32_t all = 0;
+      for (int w = 0; w < DRAW_WARPS; ++w) all += s.warp_a[w];
+      peer_put(&s.peer_match[rank], tid, all);
+    }
+    cluster_sync();                                              // and the last access to another CTA's shared memory lies ahead of it
+    if (skip) return;
+    if (empty) {
+      if (rank == 0 && tid == 0) write(0);
+      return;
+    }
+    for (int k = 0; k < rank; ++k) ahead += s.peer_match[k];
   }
-  cluster_sync();                                                // and the last access to another CTA's shared memory lies ahead of it
-  if (skip) return;
-  if (empty) {
-    if (rank == 0 && tid == 0) write(0);
-    return;
-  }
-  uint32_t ahead = 0;
-  for (int k = 0; k < rank; ++k) ahead += s.peer_match[k];
   for (int w = 0; w < warp; ++w) ahead += s.warp_a[w];
   if (taken <= ahead || taken > ahead + mine) return;
   uint32_t left = taken - ahead;                         // of the warp's
@@ -558,7 +592,7 @@ cudaError_t draw_as(const bf16* logits, long long ld, int rows, int vocab, const
     cudaError_t e = cudaFuncSetAttribute(draw_rows_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DrawShared<C>));
     if (e != cudaSuccess) { configured.forget_current_device(); return e; }
   }
-  return launch_k_cluster(C, draw_rows_kernel<C>, dim3(rows * C), dim3(DRAW_THREADS), sizeof(DrawShared<C>), s, logits, ld, vocab, settings, uniform,
+  return launch_k_cluster(C, draw_rows_kernel<C>, dim3(rows * C), dim3(draw_threads(C)), sizeof(DrawShared<C>), s, logits, ld, vocab, settings, uniform,
                           tokens, logprobs, tokens_host, logprobs_host, skip_greedy);
 }
 
@@ -568,8 +602,8 @@ cudaError_t launch_draw_rows(const bf16* logits, long long ld, int rows, int voc
                              uint32_t* tokens, float* logprobs, int sm_count, cudaStream_t s, uint32_t* tokens_host, float* logprobs_host,
                              int skip_greedy) {
   if (rows <= 0) return cudaSuccess;
-  // As many CTAs a row as the SMs hold at once, two on each, and two where the rows are more. Rows of 128256 with 1, 2, 4 and 8
-  // CTAs each: one row 22.1, 17.6, 13.9 and 13.7 us; 192 rows 46.6, 43.7, 52.9 and 94.7.
+  // As many CTAs a row as the SMs hold at once, two on each, and two where the rows are more. Rows of 128256 with 2, 4 and 8
+  // CTAs each: one row 17.6, 13.9 and 11.6 us; 192 rows 40.8, 49.2 and 94.7.
   const int room = 2 * sm_count / rows;
   auto as = room >= 8 ? draw_as<8> : room >= 4 ? draw_as<4> : draw_as<2>;
   return as(logits, ld, rows, vocab, settings, uniform, tokens, logprobs, s, tokens_host, logprobs_host, skip_greedy);
