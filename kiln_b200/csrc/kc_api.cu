@@ -162,7 +162,7 @@ struct Layer {
 
 // Per-step metadata, packed on the host and copied to the device in one transfer.
 struct MetaLayout {
-  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, sampling, uniform, shared_units, total;
+  size_t tokens, token_pos, kv_slot, sampled, tables, units, v_row_off, v_draft_off, v_draft_len, v_draft, feed, sampling, uniform, shared_units, shared_rest, total;
 };
 
 struct kc_model {
@@ -1253,11 +1253,12 @@ struct StepPlan {
   bool draws = false;              // sampled rows have settings and random numbers (kc_verify_step_sampled)
   std::vector<AttnUnit> units;
   // The same attention with the chunks that neighbours share read once (plan_shared): units of those chunks over the rows of all
-  // that share them, and units of the other chunks.
+  // that share them, and units of the other chunks. rest, where it isn't empty: the latter, for a launch behind the former's, which
+  // goes on from what that has of a chunk's first keys.
   struct Shared {
     bool on = false, keys = false;
     int tokens_per_item = 1;
-    std::vector<AttnUnit> units;
+    std::vector<AttnUnit> units, rest;
   } shared;
   MetaLayout lay{};
 };
@@ -1275,7 +1276,7 @@ void plan_attention(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>
       AttnUnit u{};
       u.seq = i; u.tok0 = row + t; u.ntok = std::min(p->tokens_per_item, s.len - t); u.pos0 = s.offset + t;
       u.chunk0 = 0; u.chunk1 = (u.pos0 + u.ntok - 1) / ATT_CHUNK + 1;
-      u.small = p->tokens_per_item > ATT_SMALL_TOKENS && u.ntok <= ATT_SMALL_TOKENS ? 1 : 0;
+      u.form = of_form(p->tokens_per_item > ATT_SMALL_TOKENS && u.ntok <= ATT_SMALL_TOKENS);
       u.old = old[i];
       items.push_back(u);
     }
@@ -1333,72 +1334,109 @@ std::vector<int> old_keys(kc_kv* kv, const kc_seq_step* seqs, int n_seqs) {
 // 32 47.5 -> 40.2, 128 rows, 6144 by 16, capped 41.7 -> 51.2.
 int shared_key_rows(int head_dim) { return head_dim > 128 ? KEY_ROWS : 2 * KEY_ROWS; }
 
+// Keys that a unit reads, and the tiles of 128 that it takes for them.
+int unit_keys(const AttnUnit& u) {
+  const int upto = u.form >> 16;
+  return std::min(upto ? u.chunk0 * ATT_CHUNK + upto * ATT_PIECE : u.chunk1 * ATT_CHUNK, u.pos0 + u.ntok) - u.chunk0 * ATT_CHUNK - (u.form >> 8 & 0xff) * ATT_PIECE;
+}
+long long unit_tiles(const std::vector<AttnUnit>& units) {
+  long long n = 0;
+  for (const AttnUnit& u : units) n += (unit_keys(u) + 127) / 128;
+  return n;
+}
+
 // Units over shared prefixes. Sequences that stand next to each other in the step and name the same blocks for a chunk, and for
 // all chunks ahead of it, are a run there; no key of the chunk is written by the step. The run's rows are taken together against
 // the chunk, as many as a unit holds, and every chunk's partial result is merged in index order as ever: a row has the bits
-// that it has alone.
+// that it has alone. Of the chunk that a prefix ends in, the pieces of 128 keys that all have in common may be taken together
+// too; each sequence's unit then goes on from there, in a second launch.
 void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& old, int block_size, int head_dim, int gqa, int kv_heads, int sm_count,
                  bool alone, bool capped) {
   StepPlan::Shared& sh = p->shared;
-  const int n = p->n_seqs, per = ATT_CHUNK / block_size;
+  const int n = p->n_seqs, per = ATT_CHUNK / ATT_PIECE;
   if (p->max_len > 16) return;   // a piece of a prompt: partial results of all its chunks would cost what is saved
-  std::vector<int> common(n + 1, 0), row(n + 1, 0);   // chunks that a sequence shares with the one before it; first row
-  int most = 0;
+  // Pieces and chunks that a sequence shares with the one before it; first row; pieces that it does not take itself.
+  std::vector<int> pieces(n + 1, 0), common(n + 1, 0), row(n + 1, 0), from(n, 0);
+  int most = 0, any = 0;
   for (int i = 0; i < n; ++i) {
     row[i + 1] = row[i] + seqs[i].len;
     if (i == 0) continue;
-    const int limit = std::min(old[i - 1], old[i]) / ATT_CHUNK;
-    int& c = common[i];
-    while (c < limit && std::equal(seqs[i].blocks + c * per, seqs[i].blocks + (c + 1) * per, seqs[i - 1].blocks + c * per)) ++c;
-    most = std::max(most, c);
+    const int limit = std::min(old[i - 1], old[i]) / block_size;
+    const int same = (int)(std::mismatch(seqs[i].blocks, seqs[i].blocks + limit, seqs[i - 1].blocks).first - seqs[i].blocks);
+    any = std::max(any, pieces[i] = (int)((long long)same * block_size / ATT_PIECE));
+    most = std::max(most, common[i] = pieces[i] / per);
   }
-  if (most == 0) return;
-  int widest = 1;   // tokens of a run
-  auto runs = [&](int c, auto&& each) {
+  if (any == 0) return;
+  // each(first sequence, first row, row behind the last one, last sequence) of the runs of neighbours that `linked` links.
+  auto runs = [&](auto&& linked, auto&& each) {
     for (int i = 0, j; i < n; i = j + 1) {
-      for (j = i; j + 1 < n && common[j + 1] > c; ++j) {}
-      if (j > i) each(i, row[i], row[j + 1]);
+      for (j = i; j + 1 < n && linked(j + 1); ++j) {}
+      if (j > i) each(i, row[i], row[j + 1], j);
     }
   };
-  runs(0, [&](int, int r0, int r1) { widest = std::max(widest, r1 - r0); });
-  sh.keys = p->tokens_per_item * gqa <= KEY_ROWS && widest * gqa <= shared_key_rows(head_dim);
-  sh.tokens_per_item = std::min(std::max(1, (sh.keys ? KEY_ROWS : ATT_ROWS) / gqa), std::max(widest, p->tokens_per_item));
-  auto small = [&](int tokens) { return sh.tokens_per_item > ATT_SMALL_TOKENS && tokens <= ATT_SMALL_TOKENS ? 1 : 0; };
+  auto own = [&](int i) { return std::max(common[i], common[i + 1]); };   // first chunk that a sequence takes by itself
+  auto partly = [&](int i) { return pieces[i] % per && common[i] == own(i) && common[i] == own(i - 1); };
+  auto partly_runs = [&](auto&& each) {
+    runs([&](int i) { return partly(i); }, [&](int i, int r0, int r1, int j) { each(i, r0, r1, j, *std::min_element(&pieces[i + 1], &pieces[j] + 1) % per); });
+  };
+  int widest = 1;   // tokens of a run
+  runs([&](int i) { return common[i] > 0; }, [&](int, int r0, int r1, int) { widest = std::max(widest, r1 - r0); });
+  const int item = p->tokens_per_item;
+  // The second launch, and its units' way into what they go on from, cost 6 to 10 us. Over 386 calls (five shapes of heads, 1 and 4 rows, 8 to
+  // 128 sequences, tails of 40 and 300) it is 0.83 of the time without where it saves 10 to 20 tiles an SM, 0.68 beyond, 0.98 at
+  // 6 to 10, 1.04 at 4 to 6, 1.3 at 1.
+  bool resumes = false;
+  if (item * gqa <= KEY_ROWS) {
+    const int per_unit = std::max(1, ATT_ROWS / gqa);
+    long long saved = 0;
+    partly_runs([&](int i, int r0, int r1, int j, int k) { saved += (long long)k * (j - i + 1 - (r1 - r0 + per_unit - 1) / per_unit); });
+    resumes = saved * kv_heads >= 8ll * sm_count;
+  }
+  if (resumes) partly_runs([&](int, int r0, int r1, int, int) { widest = std::max(widest, r1 - r0); });
+  sh.keys = item * gqa <= KEY_ROWS && widest * gqa <= shared_key_rows(head_dim);
+  sh.tokens_per_item = std::min(std::max(1, (sh.keys ? KEY_ROWS : ATT_ROWS) / gqa), std::max(widest, item));
+  auto small = [](int tokens, int box) { return box > ATT_SMALL_TOKENS && tokens <= ATT_SMALL_TOKENS; };
+  auto together = [&](int c, int k, int i, int r0, int r1) {   // all rows of a run against a chunk, or its first k pieces
+    for (int t = r0; t < r1; t += sh.tokens_per_item) {
+      AttnUnit u{};
+      u.seq = i; u.tok0 = t; u.ntok = std::min(sh.tokens_per_item, r1 - t);
+      u.pos0 = (c + 1) * ATT_CHUNK;   // every row lies past the keys
+      u.old = c * ATT_CHUNK + (k ? k * ATT_PIECE : ATT_CHUNK);
+      u.chunk0 = c; u.chunk1 = c + 1;
+      u.form = of_form(small(u.ntok, sh.tokens_per_item), 0, k);
+      sh.units.push_back(u);
+    }
+  };
   for (int c = 0; c < most; ++c)
-    runs(c, [&](int i, int r0, int r1) {
-      for (int t = r0; t < r1; t += sh.tokens_per_item) {
-        AttnUnit u{};
-        u.seq = i; u.tok0 = t; u.ntok = std::min(sh.tokens_per_item, r1 - t);
-        u.pos0 = u.old = (c + 1) * ATT_CHUNK;   // every row lies past the chunk
-        u.chunk0 = c; u.chunk1 = c + 1;
-        u.small = small(u.ntok);
-        sh.units.push_back(u);
-      }
+    runs([&](int i) { return common[i] > c; }, [&](int i, int r0, int r1, int) { together(c, 0, i, r0, r1); });
+  if (resumes)
+    partly_runs([&](int i, int r0, int r1, int j, int k) {
+      together(own(i), k, i, r0, r1);
+      std::fill(&from[i], &from[j] + 1, k);
     });
   std::vector<AttnUnit> last;
+  std::vector<AttnUnit>& others = resumes ? sh.rest : sh.units;
   for (int i = 0; i < n; ++i)
-    for (int t = 0; t < seqs[i].len; t += p->tokens_per_item) {
+    for (int t = 0; t < seqs[i].len; t += item) {
       AttnUnit u{};
-      u.seq = i; u.tok0 = row[i] + t; u.ntok = std::min(p->tokens_per_item, seqs[i].len - t); u.pos0 = seqs[i].offset + t;
-      u.small = small(u.ntok);
+      u.seq = i; u.tok0 = row[i] + t; u.ntok = std::min(item, seqs[i].len - t); u.pos0 = seqs[i].offset + t;
+      const bool few = small(u.ntok, resumes ? item : sh.tokens_per_item);
       u.old = old[i];
       const int end = (u.pos0 + u.ntok - 1) / ATT_CHUNK + 1;
-      for (int c = std::max(common[i], common[i + 1]); c < end; ++c) {
+      for (int c = own(i); c < end; ++c) {
         u.chunk0 = c; u.chunk1 = c + 1;
-        (c + 1 < end ? sh.units : last).push_back(u);
+        u.form = of_form(few, c == own(i) ? from[i] : 0);
+        (c + 1 < end && unit_keys(u) == ATT_CHUNK ? others : last).push_back(u);
       }
     }
-  std::stable_sort(last.begin(), last.end(), [](const AttnUnit& a, const AttnUnit& b) { return (a.pos0 + a.ntok - 1) % ATT_CHUNK > (b.pos0 + b.ntok - 1) % ATT_CHUNK; });
-  sh.units.insert(sh.units.end(), last.begin(), last.end());
+  std::stable_sort(last.begin(), last.end(), [](const AttnUnit& a, const AttnUnit& b) { return unit_keys(a) > unit_keys(b); });
+  others.insert(others.end(), last.begin(), last.end());
   // Tiles of 128 keys, the work of the SMs. Sharing costs 3 to 7 us more to begin with (partial results of every chunk and the kernel that
   // merges them, units of more rows). Over 384 calls (four shapes of heads, 1 and 5 rows, 2 to 64 sequences, 512 to 8192 shared keys, tails of 40
   // and 670), where it saves 3.5 tiles an SM it is up to 7.0 times as fast and at the worst 1.15 times as slow; where it saves
   // fewer, it is left out at a loss of 2 % on average.
-  long long all = 0, now = 0;
-  for (const AttnUnit& u : p->units) all += (std::min(u.chunk1 * ATT_CHUNK, u.pos0 + u.ntok) - u.chunk0 * ATT_CHUNK + 127) / 128;
-  for (const AttnUnit& u : sh.units) now += (std::min(u.chunk1 * ATT_CHUNK, u.pos0 + u.ntok) - u.chunk0 * ATT_CHUNK + 127) / 128;
-  sh.on = (all - now) * kv_heads * 2 >= 7ll * sm_count;
-  if (!sh.on) sh.units.clear();
+  sh.on = (unit_tiles(p->units) - unit_tiles(sh.units) - unit_tiles(sh.rest)) * kv_heads * 2 >= 7ll * sm_count;
+  if (!sh.on) { sh.units.clear(); sh.rest.clear(); }
 }
 
 int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, const kc_seq_step* seqs, int32_t n_seqs,
@@ -1453,7 +1491,7 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
   L.v_draft = put((size_t)n * 4);
   L.feed = put((size_t)n * 4);
   if (p.draws) { L.sampling = put((size_t)p.n_sampled * sizeof(kc_sampling)); L.uniform = put((size_t)p.n_sampled * 4); }
-  if (p.shared.on) L.shared_units = put(p.shared.units.size() * sizeof(AttnUnit));
+  if (p.shared.on) { L.shared_units = put(p.shared.units.size() * sizeof(AttnUnit)); L.shared_rest = put(p.shared.rest.size() * sizeof(AttnUnit)); }
   L.total = at;
   *plan = std::move(p);
   return KC_OK;
@@ -1487,7 +1525,10 @@ int upload_meta(kc_model* m, kc_kv* kv, const uint32_t* token_ids, const kc_seq_
   int32_t* sampled = reinterpret_cast<int32_t*>(hbuf + L.sampled);
   int32_t* tables = reinterpret_cast<int32_t*>(hbuf + L.tables);
   memcpy(hbuf + L.units, p.units.data(), p.units.size() * sizeof(AttnUnit));
-  if (p.shared.on) memcpy(hbuf + L.shared_units, p.shared.units.data(), p.shared.units.size() * sizeof(AttnUnit));
+  if (p.shared.on) {
+    std::copy(p.shared.units.begin(), p.shared.units.end(), reinterpret_cast<AttnUnit*>(hbuf + L.shared_units));
+    std::copy(p.shared.rest.begin(), p.shared.rest.end(), reinterpret_cast<AttnUnit*>(hbuf + L.shared_rest));
+  }
   int32_t* v_row = reinterpret_cast<int32_t*>(hbuf + L.v_row_off);
   int32_t* v_doff = reinterpret_cast<int32_t*>(hbuf + L.v_draft_off);
   int32_t* v_dlen = reinterpret_cast<int32_t*>(hbuf + L.v_draft_len);
@@ -1586,10 +1627,18 @@ int run_attention(kc_model* m, kc_kv* kv, const StepPlan& p, int layer, bf16* ou
     a.n_units = (int)p.shared.units.size();
     a.q_tokens = p.shared.tokens_per_item; a.keys = p.shared.keys ? 1 : 0;
     a.whole = a.single = 0;
+    a.more = p.shared.rest.empty() ? 0 : 1;
   }
   const kc_model::QMaps& q = m->q_maps[shared ? 1 : 0];
-  LAUNCH(c, KC_PROF_ATTN, a.whole || a.single ? 1 : 2,
+  LAUNCH(c, KC_PROF_ATTN, a.whole || a.single || a.more ? 1 : 2,
          paged_attention(kv->map, kv->map_one, q.map, q.small, a, in_order, kv->head_dim, p.n, c->sm_count, c->stream));
+  if (!a.more) return KC_OK;
+  a.units = reinterpret_cast<const AttnUnit*>(m->meta_dev + p.lay.shared_rest);
+  a.n_units = (int)p.shared.rest.size();
+  a.q_tokens = p.tokens_per_item;
+  a.keys = a.resumes = 1; a.more = 0;
+  const kc_model::QMaps& own = m->q_maps[0];
+  LAUNCH(c, KC_PROF_ATTN, 2, paged_attention(kv->map, kv->map_one, own.map, own.small, a, false, kv->head_dim, p.n, c->sm_count, c->stream));
   return KC_OK;
 }
 
@@ -2146,7 +2195,7 @@ static int set_attn_plan(kc_attn_plan* p, const kc_seq_step* seqs, int32_t n_seq
   for (int capped = 0; capped < 2; ++capped)
     RC(validate_step(p->shell[0], p->kv, ids.data(), (int32_t)n, seqs, n_seqs, 0, &plan[capped], true, capped != 0, false, true));
   const bool apart = plan[0].shared.on != plan[1].shared.on || plan[0].whole != plan[1].whole || !same_units(plan[0].units, plan[1].units) ||
-                     !same_units(plan[0].shared.units, plan[1].shared.units);
+                     !same_units(plan[0].shared.units, plan[1].shared.units) || !same_units(plan[0].shared.rest, plan[1].shared.rest);
   if (apart && !p->shell[1]) RC(new_shell(p->ctx, &p->shell[1]));
   if (apart) set_shell(p->shell[1], p->kv, p->num_heads, (int)n, n_seqs);
   p->plan[0].n = p->plan[1].n = 0;
@@ -2196,8 +2245,9 @@ extern "C" int kc_attn_plan_keys(kc_attn_plan_t p, int64_t* read, int64_t* apart
   if (!p || !read || !apart) return fail(KC_ERR_INVALID, "kc_attn_plan_keys: NULL argument");
   const StepPlan& plan = p->plan[0];
   int64_t r = 0, all = 0;
-  for (const AttnUnit& u : plan.shared.on ? plan.shared.units : plan.units) r += std::min(u.chunk1 * ATT_CHUNK, u.pos0 + u.ntok) - u.chunk0 * ATT_CHUNK;
-  for (const AttnUnit& u : plan.units) all += std::min(u.chunk1 * ATT_CHUNK, u.pos0 + u.ntok) - u.chunk0 * ATT_CHUNK;
+  for (const AttnUnit& u : plan.shared.on ? plan.shared.units : plan.units) r += unit_keys(u);
+  for (const AttnUnit& u : plan.shared.rest) r += unit_keys(u);
+  for (const AttnUnit& u : plan.units) all += unit_keys(u);
   *read = r;
   *apart = all;
   return KC_OK;

@@ -142,10 +142,10 @@ attn_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ C
       if (!ok) break;
       qphase ^= 1;
       if (lane == 0) {
-        const int tokens = u.small ? ATT_SMALL_TOKENS : p.q_tokens;
+        const int tokens = u.small() ? ATT_SMALL_TOKENS : p.q_tokens;
         mbar_arrive_expect_tx(q_full, S::SLABS * tokens * p.gqa * 128);
         for (int s = 0; s < S::SLABS; ++s)
-          tma_load_5d(sQ + s * ATT_ROWS * 128, u.small ? &qmap_small : &qmap, 0, 0, s, kvh, u.tok0, q_full);
+          tma_load_5d(sQ + s * ATT_ROWS * 128, u.small() ? &qmap_small : &qmap, 0, 0, s, kvh, u.tok0, q_full);
       }
       for (; u.live() && ok; u.next(TK)) {
         if (u.c != loaded_c) { loaded_c = u.c; my_blk = entries(); }
@@ -662,7 +662,7 @@ cudaError_t launch_d(const CUtensorMap& map, const CUtensorMap& kmap, const CUte
     }
     e = launch_attn<D, false>(map, q, q_small, p, in_order, sm_count, s);
   }
-  if (e != cudaSuccess || p.single) return e;
+  if (e != cudaSuccess || p.single || p.more) return e;
   const int n_rows = n_tokens * p.Hq;
   return launch_k(attn_combine_kernel<D>, dim3((n_rows + 7) / 8), dim3(256), 0, s, p, n_rows);
 }
@@ -740,7 +740,7 @@ bool make_tmap_kv_2d(CUtensorMap* map, const void* pool, uint32_t head_dim, uint
 
 cudaError_t paged_attention(const CUtensorMap& kvmap, const CUtensorMap& kmap, const CUtensorMap& qmap, const CUtensorMap& qmap_small,
                             const AttnParams& p, bool in_order, int head_dim, int n_tokens, int sm_count, cudaStream_t s) {
-  if (p.gqa < 1 || p.gqa * p.q_tokens > ATT_ROWS || p.n_units < 1) return cudaErrorInvalidValue;
+  if (p.gqa < 1 || p.gqa * p.q_tokens > ATT_ROWS || p.n_units < 1 || (p.resumes && !p.keys)) return cudaErrorInvalidValue;
   switch (head_dim) {
     case 64: return launch_d<64>(kvmap, kmap, qmap, qmap_small, p, in_order, n_tokens, sm_count, s);
     case 128: return launch_d<128>(kvmap, kmap, qmap, qmap_small, p, in_order, n_tokens, sm_count, s);

@@ -14,10 +14,14 @@ constexpr int ATT_ROWS = 128;   // query rows (token x head of the group) of one
 struct AttnUnit {
   int seq, tok0, ntok, pos0;    // sequence, first token row in the step, tokens, absolute position of the first
   int chunk0, chunk1;
-  int small;                    // 1: at most ATT_SMALL_TOKENS tokens (the query map with the small box)
+  int form;                     // of_form
   int old;                      // keys from the sequence's start that nothing in this step writes
 };
 constexpr int ATT_SMALL_TOKENS = 8;
+// AttnUnit::form. small: at most ATT_SMALL_TOKENS tokens (the query map with the small box). Of units of one chunk, in pieces of
+// ATT_PIECE keys: from: the chunk's first ones are in its partial result already; upto (0: all): no keys behind these.
+constexpr int ATT_PIECE = 128;
+constexpr int of_form(bool small, int from = 0, int upto = 0) { return (small ? 1 : 0) | from << 8 | upto << 16; }
 constexpr int KEY_ROWS = 64;    // the most rows of a unit of the kernel with a key per thread (kc_attn_keys.cu)
 
 struct AttnParams {
@@ -34,6 +38,8 @@ struct AttnParams {
   int layer, NB, BS;
   int max_chunks;
   int whole;                   // 1: every unit holds all chunks of its rows: the kernel writes `out`, no combine kernel follows
+  int resumes;                 // 1: units may go on from partial results (from > 0): attn_keys_kernel
+  int more;                    // 1: other units of the rows follow in another launch: no combine kernel behind this one
   int single;                  // 1: no row of the step has a second chunk (max_chunks == 1): no combine kernel either
   float scale;                 // softmax scale (applied to fp32 scores)
   float softcap;               // 0 = off

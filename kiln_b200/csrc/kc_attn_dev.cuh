@@ -35,13 +35,13 @@ __device__ __forceinline__ uint32_t finish2(float a, float b, const RowSum& s) {
 
 // The tiles of one unit in order, as every role walks them.
 struct UnitTiles {
-  int seq, tok0, ntok, pos0, small, old, rows, pos_max, wlo;
+  int seq, tok0, ntok, pos0, form, old, rows, pos_max, wlo;
   int c, c1, t, t1, keys;       // chunk, end of chunks, tile, end of tiles of the chunk, keys of the chunk
   __device__ __forceinline__ void open(const AttnParams& p, int unit, int tk) {
     const int4 a = *reinterpret_cast<const int4*>(&p.units[unit]);
     const int4 b = *(reinterpret_cast<const int4*>(&p.units[unit]) + 1);
     seq = a.x; tok0 = a.y; ntok = a.z; pos0 = a.w;
-    c = b.x; c1 = b.y; small = b.z; old = b.w;
+    c = b.x; c1 = b.y; form = b.z; old = b.w;
     rows = ntok * p.gqa;
     pos_max = pos0 + ntok - 1;
     wlo = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;    // first key that any row of the unit sees
@@ -49,13 +49,15 @@ struct UnitTiles {
     chunk(tk);
   }
   __device__ __forceinline__ void chunk(int tk) {
-    keys = min(ATT_CHUNK, pos_max + 1 - c * ATT_CHUNK);
-    t = max(0, wlo - c * ATT_CHUNK) / tk;
+    keys = min(form >> 16 ? (form >> 16) * ATT_PIECE : ATT_CHUNK, pos_max + 1 - c * ATT_CHUNK);
+    t = first_tile(tk);
     t1 = (keys + tk - 1) / tk;
   }
   __device__ __forceinline__ bool live() const { return c < c1; }
   __device__ __forceinline__ bool last() const { return t == t1 - 1; }
-  __device__ __forceinline__ int first_tile(int tk) const { return max(0, wlo - c * ATT_CHUNK) / tk; }
+  __device__ __forceinline__ bool small() const { return form & 1; }
+  __device__ __forceinline__ int from() const { return (form >> 8 & 0xff) * ATT_PIECE; }
+  __device__ __forceinline__ int first_tile(int tk) const { return max(from(), wlo - c * ATT_CHUNK) / tk; }
   __device__ __forceinline__ int key0(int tk) const { return c * ATT_CHUNK + t * tk; }
   // 16-key blocks of the tile that hold a key of the sequence
   __device__ __forceinline__ int blocks(int tk) const { return (min(tk, keys - t * tk) + 15) >> 4; }

@@ -24,6 +24,7 @@
 #include "kc_attn_dev.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace kc {
 
@@ -92,7 +93,9 @@ __device__ __forceinline__ void cross_warps(int set) { asm volatile("bar.sync %0
 // costs a fetch of instructions behind it.
 enum { PLAIN, CAPPED, SCALED };
 
-template <int D, int NR, int MODE>
+// RESUMES: units may go on from the partial result of their chunk's first keys (AttnUnit::form), with the same bits as if they had
+// begun it: (m, l) into the softmax warps' registers, O into tensor memory ahead of the first product.
+template <int D, int NR, int MODE, bool RESUMES>
 __global__ void __launch_bounds__(KEY_THREADS, 1)
 attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ CUtensorMap qmap,
                  const __grid_constant__ CUtensorMap qmap_small, const AttnParams p) {
@@ -116,7 +119,8 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
   uint64_t* stat_full = pv_done + 2;    // [2] (m, l) of a chunk; with the last PV of the chunk its O is complete
   uint64_t* o_full = stat_full + 2;
   uint64_t* o_empty = o_full + 2;       // [2] O and (m, l) have been read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+  uint64_t* o_loaded = o_empty + 2;     // the partial results that a unit goes on from are in O
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_loaded + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -125,7 +129,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
   fence_proxy_async_smem();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::RING; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
-    mbar_init(q_full, 1); mbar_init(q_empty, 1);
+    mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(o_loaded, 4 * KEY_SETS);
     for (int i = 0; i < 2; ++i) { mbar_init(&s_ready[i], 1); mbar_init(&p_ready[i], 4 * KEY_SETS); mbar_init(&pv_done[i], 1); mbar_init(&stat_full[i], KEY_SETS); mbar_init(&o_full[i], 1); mbar_init(&o_empty[i], 4); }
     mbar_fence_init();
   }
@@ -169,10 +173,10 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
         if (!ok) return;
         qphase ^= 1;
         if (lane == 0) {
-          const int tokens = u.small ? ATT_SMALL_TOKENS : p.q_tokens;
+          const int tokens = u.small() ? ATT_SMALL_TOKENS : p.q_tokens;
           mbar_arrive_expect_tx(q_full, S::SLABS * tokens * p.gqa * 128);
           for (int s = 0; s < S::SLABS; ++s)
-            tma_load_5d(sQ + s * NR * 128, u.small ? &qmap_small : &qmap, 0, 0, s, kvh, u.tok0, q_full);
+            tma_load_5d(sQ + s * NR * 128, u.small() ? &qmap_small : &qmap, 0, 0, s, kvh, u.tok0, q_full);
         }
         __syncwarp();
       };
@@ -227,7 +231,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
     uint32_t qphase = 0;
     bool ok = true;
     // the tile whose PV is still to be issued
-    bool pend = false, pend_first = false, pend_last = false;
+    bool pend = false, pend_first = false, pend_last = false, pend_resumed = false;
     int pend_nb = 0, pend_tile = 0, pend_chunk = 0;
     RingPos pend_v;
     auto issue_pv = [&]() {
@@ -242,7 +246,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
       if (elect_one()) {
         for (int b = 0; b < pend_nb; ++b) {
           const uint32_t vb = v_lo + b * (2 * S::GROUP_BYTES >> 4), pb = p_lo + b * (16 * 128 >> 4);
-          const uint32_t acc = pend_first && b == 0 ? 0u : 1u;
+          const uint32_t acc = pend_first && b == 0 && !(RESUMES && pend_resumed) ? 0u : 1u;
 #pragma unroll
           for (int h = 0; h < H; ++h) {
             umma_bf16_ss(o + h * NR, vb + h * (2 * 1024 >> 4), v_hi, pb, p_hi, idesc_pv, acc);
@@ -283,7 +287,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
         first_of_unit = false;
         tc_fence_after();
         const int nb = u.blocks(TK), sb = tile & 1, stage = kv.stage, chunk = chunks;
-        const bool first = u.t == u.first_tile(TK), last = u.last();
+        const bool first = u.t == u.first_tile(TK), last = u.last(), resumed = RESUMES && u.from() > 0;
         if (last) ++chunks;
         u.next(TK);
         const bool unit_done = !u.live();
@@ -299,7 +303,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
         __syncwarp();
         kv.advance(S::RING);
         if (pend) issue_pv();
-        pend = true; pend_first = first; pend_last = last; pend_nb = nb; pend_tile = tile; pend_chunk = chunk; pend_v = kv;
+        pend = true; pend_first = first; pend_last = last; pend_nb = nb; pend_tile = tile; pend_chunk = chunk; pend_v = kv; pend_resumed = resumed;
         kv.advance(S::RING);
         ++tile;
       }
@@ -320,6 +324,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
     constexpr int ODD = KEY_SETS * 4 * 16;
     const int row = (set + KEY_SETS * (lane >> 3)) * 8 + (lane & 7), slot = lane & 15;
     int tile = 0, chunks = 0;
+    uint32_t loaded_phase = 0;
     bool ok = true;   // once false: no more waits, but the crossings
     for (int r0 = 0, w; r0 * (int)gridDim.x < total; ++r0) {
       if ((w = unit_index(r0, blockIdx.x, gridDim.x, total)) < 0) break;
@@ -330,6 +335,40 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
       const bool row_live = row < u.rows && lane < 16;
       const int pos = u.pos0 + min(row / p.gqa, u.ntok - 1);
       float m = -INFINITY, l = 0.f, alpha = 1.f;
+      const bool resumed = RESUMES && u.from() > 0;
+      float2 before = make_float2(-INFINITY, 0.f);
+      if (resumed) {
+        // where row r of the unit has its partial result: for every kv head the rows are (token, head of the group)
+        const auto at = [&](int r) {
+          const int t = r / p.gqa;
+          return ((size_t)(u.tok0 + t) * p.Hq + (w % p.Hkv) * p.gqa + (r - t * p.gqa)) * p.max_chunks + u.c;
+        };
+        if (row_live) before = __ldcg(&p.part_ml[at(row)]);
+        // The buffer's last chunk has been read; and no set is still to begin the last such unit, whose arrivals would be taken for these.
+        ok = ok && warp_wait(&o_empty[chunks & 1], ((chunks >> 1) & 1) ^ 1, p.status, KC_DEV_ATTN | 0x2f) &&
+             warp_wait(o_loaded, loaded_phase ^ 1, p.status, KC_DEV_ATTN | 0x31);
+        if (ok && has_features) {
+          tc_fence_after();
+          const uint32_t o_addr = tmem + lane_addr + S::TMEM_O + (chunks & 1) * H * NR;
+          // by the next set, which has no rows where there are few and is here ahead of the set that has them
+#pragma unroll 1
+          for (int g = (set + 1) % KEY_SETS; g < groups; g += KEY_SETS) {
+            uint32_t o[H][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float* from = p.part_o + at(min(g * 8 + j, u.rows - 1)) * D + quarter * 32 + lane;
+#pragma unroll
+              for (int h = 0; h < H; ++h) o[h][j] = __float_as_uint(__ldcg(from + h * 128));
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h) tmem_st8(o_addr + h * NR + g * 8, o[h]);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_loaded);
+      }
       // the sums of a tile, once every warp's are there
       auto add_sums = [&](int t) {
         const float* s = sum0 + (t & 1) * ODD + slot;
@@ -384,7 +423,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
           }
         }
         cross_warps(set);
-        if (first) { m = -INFINITY; l = 0.f; }
+        if (first) { m = before.x; l = before.y; }
         else add_sums(tile - 1);
         // ---- a row's maximum over the tile, its reference and what that rescales: every warp for itself ----
         const float* s = max0 + (tile & 1) * ODD + slot;
@@ -400,13 +439,14 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
         alpha = 1.f;
         if (tmax > m + 8.f) { alpha = ex2(m - tmax); m = tmax; }   // the reference lags: see attn_kernel
         if (lane < 16) my_ref[lane] = m == -INFINITY ? -0.f : -m;
-        const bool rescale = __any_sync(0xffffffffu, row_live && alpha != 1.f) && !first;
+        const bool rescale = __any_sync(0xffffffffu, row_live && alpha != 1.f) && (!first || resumed);
         __syncwarp();   // the references are there
         // ---- the products are in: of the tile whose probabilities are replaced, and of the last one where O is rescaled ----
         if (S::P_BUFS == 1 && tile > 0) ok = ok && warp_wait(&pv_done[sb ^ 1], ((tile - 1) >> 1) & 1, p.status, KC_DEV_ATTN | 0x2a);
         if (S::P_BUFS == 2 && tile > 1) ok = ok && warp_wait(&pv_done[sb], ((tile >> 1) & 1) ^ 1, p.status, KC_DEV_ATTN | 0x2a);
         if (ok && rescale && has_features) {
           ok = warp_wait(&pv_done[sb ^ 1], ((tile - 1) >> 1) & 1, p.status, KC_DEV_ATTN | 0x2c);
+          if (RESUMES && first) ok = ok && warp_wait(o_loaded, loaded_phase, p.status, KC_DEV_ATTN | 0x30);
           tc_fence_after();
           if (works) tmem_wait_ld();   // keeps x apart from what follows
           const uint32_t o_addr = tmem + lane_addr + S::TMEM_O + (chunks & 1) * H * NR;
@@ -501,6 +541,7 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
           ++chunks;
         }
       }
+      if (resumed) loaded_phase ^= 1;
     }
   } else if (warp >= 8) {
     // ---- a finished chunk: thread = feature 32 * (warp & 3) + lane, and that 128 further on. What a unit of whole rows has
@@ -627,24 +668,28 @@ attn_keys_kernel(const __grid_constant__ CUtensorMap kvmap, const __grid_constan
   }
 }
 
-template <int D, int NR, int MODE>
+template <int D, int NR, int MODE, bool RESUMES>
 cudaError_t launch_keys_as(const CUtensorMap& kv, const CUtensorMap& q, const CUtensorMap& q_small, const AttnParams& p, bool in_order,
                            int sm_count, cudaStream_t s) {
   using S = KeyShape<D, NR>;
   static DeviceOnce configured;   // the attribute belongs to the device's copy of the kernel
   if (configured.first_on_current_device()) {
-    cudaError_t e = cudaFuncSetAttribute(attn_keys_kernel<D, NR, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(attn_keys_kernel<D, NR, MODE, RESUMES>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) { configured.forget_current_device(); return e; }
   }
   const int grid = std::min(p.n_units * p.Hkv, sm_count);
-  return launch_k_opt(!in_order, attn_keys_kernel<D, NR, MODE>, dim3(grid), dim3(KEY_THREADS), S::SMEM, s, kv, q, q_small, p);
+  return launch_k_opt(!in_order, attn_keys_kernel<D, NR, MODE, RESUMES>, dim3(grid), dim3(KEY_THREADS), S::SMEM, s, kv, q, q_small, p);
 }
 template <int D, int NR>
 cudaError_t launch_keys(const CUtensorMap& kv, const CUtensorMap& q, const CUtensorMap& q_small, const AttnParams& p, bool in_order, bool folded,
                         int sm_count, cudaStream_t s) {
-  if (!folded) return launch_keys_as<D, NR, SCALED>(kv, q, q_small, p, in_order, sm_count, s);
-  return p.softcap > 0.f ? launch_keys_as<D, NR, CAPPED>(kv, q, q_small, p, in_order, sm_count, s)
-                         : launch_keys_as<D, NR, PLAIN>(kv, q, q_small, p, in_order, sm_count, s);
+  auto as = [&](auto resumes) {
+    constexpr bool R = decltype(resumes)::value;
+    if (!folded) return launch_keys_as<D, NR, SCALED, R>(kv, q, q_small, p, in_order, sm_count, s);
+    return p.softcap > 0.f ? launch_keys_as<D, NR, CAPPED, R>(kv, q, q_small, p, in_order, sm_count, s)
+                           : launch_keys_as<D, NR, PLAIN, R>(kv, q, q_small, p, in_order, sm_count, s);
+  };
+  return p.resumes ? as(std::true_type()) : as(std::false_type());
 }
 template <int D>
 cudaError_t launch_keys_d(const CUtensorMap& kv, const CUtensorMap& q, const CUtensorMap& q_small, const AttnParams& p, bool in_order, bool folded,

@@ -106,10 +106,10 @@ def test_rows_have_the_bits_that_they_have_alone(ctx, heads, kv_heads, dim, name
 
 
 @pytest.mark.parametrize("groups", [
-    [(512, [(1, 512), (1, 600)])], [(0, [(1, 900), (1, 800)])], [(496, [(1, 900 + i) for i in range(200)])], [(2000, [(4, 2040)])], [(0, [(1, 0)])],
+    [(512, [(1, 512), (1, 600)])], [(0, [(1, 900), (1, 800)])], [(112, [(1, 900 + i) for i in range(200)])], [(2000, [(4, 2040)])], [(0, [(1, 0)])],
     [(1024, [(130, 1024)] + [(1, 1200 + i) for i in range(90)])]])
 def test_what_is_not_shared(ctx, groups):
-    """Too little to be read once, less than a chunk, one sequence, no history, beside a piece of a prompt."""
+    """Too little to be read once, less than 128 keys, one sequence, no history, beside a piece of a prompt."""
     seqs, total = tables(groups, 16, 1)
     kv, data = pools(ctx, 4, 128, total, 16, 5)
     q, got, plan = run_both(ctx, kv, data, 16, seqs, 7)
@@ -160,6 +160,41 @@ def test_one_table_for_all(ctx, early):
     q, got, plan = run_both(ctx, kv, data, 8, seqs, 3)
     assert shares(plan) != early
     close(got, formula(data[0], q, seqs, 128 ** -0.5, 0.0))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (28, 4, 128), (32, 8, 64), (16, 8, 256), (64, 8, 128)])
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("prefix", [300, 511, 2048 + 130, 2048 + 400, 4096 + 511])
+def test_a_prefix_that_ends_inside_a_chunk(ctx, heads, kv_heads, dim, rows, prefix):
+    """The pieces of 128 keys that all have of the chunk are taken once, and every sequence goes on from there: in the middle of
+    a maximum's life, of a sum and of an output. In two groups, one of single rows."""
+    tails = np.random.default_rng(prefix).integers(1, 130, 390)
+    tails[:4] = 1, 128, 512, 1100
+    seqs, total = tables([(prefix // 16 * 16, [(rows, prefix + int(t)) for t in tails[:250]]), (prefix // 16 * 16, [(1, prefix + int(t)) for t in tails[250:]])], 16, 1)
+    kv, data = pools(ctx, kv_heads, dim, total, 16, 4)
+    for softcap in (0.0, 30.0):
+        q, got, plan = run_both(ctx, kv, data, heads, seqs, 3, softcap)
+        read, apart = plan.keys()
+        pieces, per = prefix // 16 * 16 // 128, 128 // (heads // kv_heads)
+        assert apart - read == pieces * 128 * (390 - -(-250 * rows // per) - -(-140 // per))
+        close(got[: 5 * rows], formula(data[0], q[: 5 * rows], seqs[:5], dim ** -0.5, softcap))
+    assert ctx.device_status() == 0
+
+
+def test_scores_that_grow_behind_a_shared_piece(ctx):
+    """The maximum of what is shared is outweighed by far behind it, and the other way round: what was summed before is scaled down, or
+    what follows."""
+    seqs, total = tables([(2048 + 256, [(1, 2048 + 256 + i) for i in range(160)])], 16, 1)
+    own = sorted({int(b) for s in seqs for b in s.blocks[(2048 + 256) // 16:]})
+    for loud, std in ((1.0, 0.05), (1.0, 40.0), (30.0, 1.0), (1 / 30, 1.0)):
+        kv, data = pools(ctx, 8, 128, total, 16, 4, std=std)
+        data[0, 0, own] *= loud            # their own keys
+        k, v = (t.transpose(1, 2).reshape(-1, 8 * 128) for t in data[0])
+        api.rope_kv_write(ctx, kv, 0, torch.cat([k, k, v], 1), torch.zeros(64, device="cuda"), 8, [api.SeqStep(total * 16, 0, 0, np.arange(total, dtype=np.uint32))])
+        q, got, plan = run_both(ctx, kv, data, 32, seqs, 3, std=1.5)
+        read, apart = plan.keys()
+        assert apart - read == (2048 + 256) * (160 - 5)
+        close(got, formula(data[0], q, seqs, 128 ** -0.5, 0.0))
 
 
 def test_windows_layers_streams_and_graphs(ctx):
