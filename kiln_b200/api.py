@@ -207,7 +207,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 def _expect(ctx: "Context", name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
     """A contiguous tensor of that type and shape on the context's device, or ValueError (cheap tests: this runs per call of
     an operator that takes a few microseconds)."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda or t.get_device() != ctx.device:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != ctx.device or not t.is_contiguous():   # -1: not on a device
         raise ValueError(f"{name}: contiguous {dtype} {list(shape)} on cuda:{ctx.device}")
 
 
@@ -581,16 +581,18 @@ def sample_rows(ctx: Context, logits: torch.Tensor, params, uniforms: torch.Tens
     rows, vocab = logits.shape
     if not isinstance(params, torch.Tensor):
         params = pack_sampling(params, logits.device)
-    if out is None:
-        out = logits.new_empty(rows, dtype=torch.int32)
-    if logprobs is None:
-        logprobs = logits.new_empty(rows, dtype=torch.float32)
-    _expect(ctx, "params", params, torch.int32, (rows, 4))
-    _expect(ctx, "uniforms", uniforms, torch.float32, (rows,))
-    _expect(ctx, "out", out, torch.int32, (rows,))
-    _expect(ctx, "logprobs", logprobs, torch.float32, (rows,))
     if logits.get_device() != ctx.device:
         raise ValueError(f"logits: on cuda:{ctx.device}")
+    _expect(ctx, "params", params, torch.int32, (rows, 4))
+    _expect(ctx, "uniforms", uniforms, torch.float32, (rows,))
+    if out is None:
+        out = logits.new_empty(rows, dtype=torch.int32)
+    else:
+        _expect(ctx, "out", out, torch.int32, (rows,))
+    if logprobs is None:
+        logprobs = torch.empty_like(uniforms)
+    else:
+        _expect(ctx, "logprobs", logprobs, torch.float32, (rows,))
     ctx.on_current_stream(L.lib().kc_sample_rows, ctx._h, logits.data_ptr(), logits.stride(0), rows, vocab, params.data_ptr(), uniforms.data_ptr(),
                           out.data_ptr(), logprobs.data_ptr())
     return out, logprobs
@@ -664,12 +666,13 @@ class Adapters:
     def apply(self, x: torch.Tensor, rows: AdapterRows, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """y + scale B (A x), row by row: x bf16 [m, in], y bf16 [m, out] (a projection's output), ``out`` for the result (y itself: in
         place). Part of torch's current stream (Context.on_current_stream); the host does not wait."""
-        if out is None:
-            out = torch.empty_like(y)
         m = rows.rows
         _expect(self.ctx, "x", x, torch.bfloat16, (m, self.in_features))
         _expect(self.ctx, "y", y, torch.bfloat16, (m, self.out_features))
-        _expect(self.ctx, "out", out, torch.bfloat16, (m, self.out_features))
+        if out is None:
+            out = torch.empty_like(y)
+        else:
+            _expect(self.ctx, "out", out, torch.bfloat16, (m, self.out_features))
         self.ctx.on_current_stream(L.lib().kc_adapters_apply, self._h, rows._h, x.data_ptr(), y.data_ptr(), out.data_ptr())
         return out
 
@@ -811,10 +814,11 @@ class AttentionPlan:
         if not self._h or not self.kv._h:
             raise ValueError("the plan or its pools are closed")
         dim = self.kv.spec.head_dim
-        if out is None:
-            out = q.new_empty(self.tokens, self.heads * dim, dtype=torch.bfloat16)
         _expect(self.ctx, "q", q, torch.bfloat16, (self.tokens, self.heads, dim))
-        _expect(self.ctx, "out", out, torch.bfloat16, (self.tokens, self.heads * dim))
+        if out is None:
+            out = q.new_empty(self.tokens, self.heads * dim)
+        else:
+            _expect(self.ctx, "out", out, torch.bfloat16, (self.tokens, self.heads * dim))
         self.ctx.on_current_stream(L.lib().kc_attn_plan_run, self._h, layer, q.data_ptr(), scale, softcap, window, out.data_ptr())
         return out
 

@@ -161,6 +161,13 @@ def test_rows_do_not_hang_on_their_number(ctx):
         assert torch.equal(got, want[:n]) and torch.equal(q.view(torch.int32), p[:n].view(torch.int32))
 
 
+@pytest.mark.parametrize("rows,vocab", [(160, 270001), (80, 530003), (1, 1048569), (1, 1200000)])
+def test_long_rows(ctx, rows, vocab):
+    """More values than a bin has room to say where they stand (8 to the vector, 16384 vectors a CTA), and just as many."""
+    rng = np.random.default_rng(vocab)
+    check(ctx, language(rows, vocab, 3)[: rows], mixed(rows, rng), rng.random(rows).astype(np.float32).clip(0, 1 - 2 ** -24).tolist())
+
+
 @pytest.mark.parametrize("rows,vocab", [(310, 50001), (310, 4099), (90, 4099), (40, 257), (1, 8)])
 def test_every_run_counts_every_token(ctx, rows, vocab):
     """The same rows many times over: a token that one run did not count would show in the log probability."""
