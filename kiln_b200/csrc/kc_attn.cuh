@@ -10,7 +10,8 @@ namespace kc {
 constexpr int ATT_CHUNK = 512;
 constexpr int ATT_ROWS = 128;   // query rows (token x head of the group) of one work item: the lanes of tensor memory
 
-// One unit of work for every kv head: consecutive tokens of one sequence against the chunks [chunk0, chunk1).
+// One unit of work for every kv head: consecutive tokens of one sequence, or of several that have the same keys there, against
+// the chunks [chunk0, chunk1).
 struct AttnUnit {
   int seq, tok0, ntok, pos0;    // sequence, first token row in the step, tokens, absolute position of the first
   int chunk0, chunk1;
