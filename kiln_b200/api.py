@@ -445,7 +445,7 @@ class CudaModel:
         row. Returns (row_tokens[n_sampled], n_committed[n_seqs], n_accepted[n_seqs], logprobs[n_sampled])."""
         p = _PackedStep(batch)
         n_sampled = sum(s.sample_rows for s in batch.seqs)
-        u = np.ascontiguousarray(uniforms, dtype=np.float32)
+        u = _uniforms(uniforms)
         if len(sampling) != p.n_seqs or u.shape != (n_sampled,):
             raise ValueError(f"{p.n_seqs} sequences and {n_sampled} sampled rows have {len(sampling)} settings and random numbers {u.shape}")
         settings = (L.KcSampling * max(1, p.n_seqs))(*[L.KcSampling(s.temperature, s.top_k, s.top_p, s.min_p) for s in sampling])
@@ -568,6 +568,14 @@ def pack_sampling(params: Sequence[SamplingParams], device) -> torch.Tensor:
     """The settings of a batch's rows as sample_rows takes them, int32 [rows, 4] on the device: made once, kept while they hold."""
     rec = np.array([(p.temperature, p.top_k, p.top_p, p.min_p) for p in params], dtype=_SAMPLING)
     return torch.from_numpy(rec.view(np.int32).reshape(-1, 4)).to(device)
+
+
+def _uniforms(values) -> np.ndarray:
+    """Random numbers as float32; one below 1 that would round to it is the number ahead of it."""
+    v = np.asarray(values, dtype=np.float64)
+    u = np.ascontiguousarray(v, dtype=np.float32)
+    u[(v < 1) & (u == 1)] = np.nextafter(np.float32(1), np.float32(0))
+    return u
 
 
 def sample_rows(ctx: Context, logits: torch.Tensor, params, uniforms: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -709,18 +717,20 @@ class QuantizedWeight:
         what they add to y (Adapters.apply)."""
         assert x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[1] == self.in_features
         m = x.shape[0]
+        if (adapters is None) != (rows is None) or adapters is not None and (
+                adapters.ctx is not self.ctx or rows.rows != m or (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features)):
+            raise ValueError("adapters of another projection or context, or not a slot for every row")
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
         y = torch.empty(m, self.out_features, dtype=torch.bfloat16, device=x.device)
         torch.cuda.current_stream().synchronize()
         check(L.lib().kc_quantized_matmul(self.ctx._h, self._h, x.data_ptr(), m, y.data_ptr()))
-        if adapters is not None:
-            if rows is None or adapters.ctx is not self.ctx or rows.rows != m or (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
-                self.ctx.sync()
-                raise ValueError("adapters of another projection or context, or not a slot for every row")
-            check(L.lib().kc_adapters_apply(adapters._h, rows._h, x.data_ptr(), y.data_ptr(), y.data_ptr()))
-        self.ctx.sync()
+        try:
+            if adapters is not None:
+                check(L.lib().kc_adapters_apply(adapters._h, rows._h, x.data_ptr(), y.data_ptr(), y.data_ptr()))
+        finally:
+            self.ctx.sync()              # x and y are not given back under the product
         return y
 
     def matmul_stream(self, x: torch.Tensor) -> torch.Tensor:
@@ -798,6 +808,8 @@ class AttentionPlan:
     def set(self, seqs: Sequence[SeqStep]) -> None:
         """Another step in the plan's place, behind the runs queued before: a generation keeps one plan and sets it every step.
         Refused once a graph has been captured over a run."""
+        if not self._h or not self.kv._h:
+            raise ValueError("the plan or its pools are closed")
         p = _PackedStep(StepBatch([], seqs))
         check(L.lib().kc_attn_plan_set(self._h, p.seq_arr, p.n_seqs))
         self.tokens = sum(s.len for s in seqs)

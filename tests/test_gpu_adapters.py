@@ -161,6 +161,11 @@ def test_beside_a_quantised_projection(ctx):
     for bad in (dict(adapters=ad), dict(adapters=ad, rows=api.AdapterRows(ctx, slots[:3])), dict(adapters=api.Adapters(ctx, 512, 64, 1, 4), rows=rows)):
         with pytest.raises(ValueError):
             weight.matmul(x, **bad)
+    with pytest.raises(ValueError):
+        weight.matmul(x, rows=rows)
+    ad.close()
+    with pytest.raises(api.KcError):
+        weight.matmul(x, ad, rows)
     assert torch.equal(weight.matmul(x), plain)
 
 

@@ -344,9 +344,11 @@ def test_refusals(ctx):
     plan.run(0, q, 1.0)
     ctx.sync()
     kv.close()
-    with pytest.raises(ValueError):
-        plan.run(0, q, 1.0)
+    for call in (lambda: plan.run(0, q, 1.0), lambda: plan.set(good)):
+        with pytest.raises(ValueError):
+            call()
     plan.close()
-    with pytest.raises(ValueError):
-        plan.run(0, q, 1.0)
+    for call in (lambda: plan.run(0, q, 1.0), lambda: plan.set(good)):
+        with pytest.raises(ValueError):
+            call()
     assert api.live_objects() == live

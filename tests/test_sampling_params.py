@@ -23,6 +23,12 @@ def test_packed_settings_are_the_structs():
     assert api.pack_sampling([], "cpu").shape == (0, 4)
 
 
+def test_random_numbers_stay_below_one():
+    u = api._uniforms([0.0, 0.25, 1 - 2.0 ** -53, 1 - 2.0 ** -24, 1.0, -1.0, math.nan])
+    assert u.dtype == np.float32 and u.tolist()[:6] == [0.0, 0.25, 1 - 2.0 ** -24, 1 - 2.0 ** -24, 1.0, -1.0] and math.isnan(u[6])
+    assert api._uniforms([]).shape == (0,)
+
+
 def test_calls_are_refused_before_a_launch(fake):  # noqa: F811
     run(fake, """
 fake.fake_reset()
