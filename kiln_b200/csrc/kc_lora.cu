@@ -1,7 +1,7 @@
 // What low-rank adapters add to a projection's rows: out_i = y_i + s_a B_a (A_a x_i), a the adapter of row i.
 //
 // One launch. Rows are grouped by adapter on the host (kc_adapter_rows_create) into tiles of at most 16, and a tile is a cluster's
-// of eight, four or two CTAs: each multiplies its share of the features of x with A's columns, the partial t = A x [rows, rank] meet
+// of two to eight CTAs: each multiplies its share of the features of x with A's columns, the partial t = A x [rows, rank] meet
 // in the cluster's shared memory, and each CTA takes its share of the projection's features through B and adds them to y. So t
 // never goes through memory, and no workspace or order of atomics is involved.
 //
@@ -60,7 +60,7 @@ __device__ __forceinline__ void load_regs(uint32_t* r, const void* from) {
 template <int CTAS_, int R_>
 struct LoraShape {
   static constexpr int CTAS = CTAS_, R = R_, ROWS = LORA_TILE;
-  static constexpr int PARTS = 8 / CTAS;           // eighths of the features of x that a CTA has
+  static constexpr int PARTS = (7 + CTAS) / CTAS;  // eighths of the features of x that a CTA has, at the most
   static constexpr int RS = R < 64 ? R : 64;       // ranks of a step of the first product
   static constexpr int PAD = R + 8;                // of a row of t: 16-byte pieces of neighbouring rows lie in different banks
   static constexpr int PART = RS + 4;
@@ -140,8 +140,9 @@ lora_kernel(const LoraParams p) {
   {
     const int chunks = p.n_in / 32, used = (slot.rank + RS - 1) / RS;   // steps of ranks in use
     const bf16 *x0 = p.x + (size_t)rows[g] * p.n_in + t * 8, *x1 = p.x + (size_t)rows[g + 8] * p.n_in + t * 8;
-    for (int i = 0; i < PARTS; ++i) {
-      const int me = (rank * PARTS + i) * LORA_WARPS + warp;
+    const int part0 = rank * 8 / CTAS, part1 = (rank + 1) * 8 / CTAS;
+    for (int i = 0; i < part1 - part0; ++i) {
+      const int me = (part0 + i) * LORA_WARPS + warp;
       const int c0 = (int)((long long)chunks * me / (8 * LORA_WARPS)), c1 = (int)((long long)chunks * (me + 1) / (8 * LORA_WARPS));
       for (int s = 0; s < used; ++s) {
         const bf16* a = p.a + ((size_t)tile.slot * R + s * RS + g) * p.n_in + t * 8;
@@ -190,7 +191,10 @@ lora_kernel(const LoraParams p) {
       if (r < slot.rank) {
         float q[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = peer_float(&sum[(k % PARTS * ROWS + row) * R + r], k / PARTS);
+        for (int k = 0; k < 8; ++k) {
+          const int owner = ((k + 1) * CTAS - 1) / 8;
+          q[k] = peer_float(&sum[((k - owner * 8 / CTAS) * ROWS + row) * R + r], owner);
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) v += q[k];
         v *= slot.scale;
@@ -268,14 +272,18 @@ cudaError_t launch(const LoraParams& p, cudaStream_t s) {
 }
 
 // The largest clusters of which the SMs hold all at once (a cluster lies in one group of SMs: of 296 places for CTAs clusters of eight
-// take 256, of four 284), else two CTAs a tile, whose fixed part weighs least. Rank 16, 4096 -> 28672 features, with 8, 4 and 2 CTAs,
-// us: 32 tiles 19.3, 24.7, 39.8; 34 28.3, 26.2, 40.0; 70 45.6, 33.4, 44.8; 74 46.9, 50.4, 45.6; 4096 -> 4096: 7.0, 7.6, 10.7; 10.3, 8.5,
-// 10.8; 18.2, 11.0, 14.4; 19.0, 16.4, 14.3.
+// take 256, of seven and six 252, of four 284, of three 270), else two CTAs a tile, whose fixed part weighs least. 4096 -> 28672 features,
+// rank 16, us with 8, 7, 6, 4, 3 and 2 CTAs: 32 tiles 11.7, 13.1, 13.9, -, -, -; 34 17.6, 14.0, 14.7; 38 20.3, 21.7, 15.2, 18.3; 46 -, 26.8, 27.1, 21.3; 72
+// -, -, -, 44.6, 34.7, 41; 94 -, -, -, -, 57.6, 44.9. Clusters of five gain 8 % on four at 46 to 53 tiles.
 template <int R>
 cudaError_t launch_rank(const LoraParams& p, int sm_count, cudaStream_t s) {
   const long long places = (long long)sm_count * LoraShape<8, R>::RESIDENT;
-  if (p.n_tiles * 8 <= places * 87 / 100) return launch<LoraShape<8, R>>(p, s);
-  if (p.n_tiles * 4 <= places * 96 / 100) return launch<LoraShape<4, R>>(p, s);
+  auto fit = [&](int ctas, int percent) { return p.n_tiles * 100ll * ctas <= places * percent; };
+  if (fit(8, 87)) return launch<LoraShape<8, R>>(p, s);
+  if (fit(7, 86)) return launch<LoraShape<7, R>>(p, s);
+  if (fit(6, 86)) return launch<LoraShape<6, R>>(p, s);
+  if (fit(4, 96)) return launch<LoraShape<4, R>>(p, s);
+  if (fit(3, 92)) return launch<LoraShape<3, R>>(p, s);
   return launch<LoraShape<2, R>>(p, s);
 }
 

@@ -69,7 +69,7 @@ def test_rows_take_their_adapters(ctx, n_in, n_out, ranks):
 
 @pytest.mark.parametrize("m,used", [(64, 1), (65, 1), (300, 2), (1000, 3), (2048, 8), (2050, 1)])
 def test_many_rows(ctx, m, used):
-    """Tiles of 16, 32 and 64 rows, the last ones in part; every row once."""
+    """Tiles of 16 rows, the last ones in part; every row once."""
     ad, parts = bank(ctx, 256, 264, [24] * used, m)
     slots = np.sort(np.random.default_rng(m).integers(0, used, m))
     x, y = inputs(m, 256, 264, m)
@@ -90,6 +90,23 @@ def test_a_row_does_not_hang_on_the_others(ctx):
     some = ad.apply(x[order].contiguous(), api.AdapterRows(ctx, slots[order]), y[order].contiguous())
     torch.cuda.synchronize()
     assert torch.equal(some, all_rows[torch.from_numpy(order).cuda()])
+
+
+@pytest.mark.parametrize("n_in,n_out,rank", [(96, 41, 16), (1024, 1032, 30), (1024, 520, 64), (2080, 264, 128)])
+def test_every_size_of_cluster(ctx, n_in, n_out, rank):
+    """Tiles by the dozen and by the hundred, whose clusters have eight to two CTAs: a row's bits are the same in all."""
+    ad, parts = bank(ctx, n_in, n_out, [rank] * 3, 1)
+    x, y = inputs(16 * 150, n_in, n_out, 2)
+    slots = np.repeat(np.arange(150) % 3, 16)
+    want, off = formula(parts, x, y, slots)
+    before = None
+    for tiles in (1, 8, 16, 17, 18, 20, 21, 33, 35, 36, 40, 42, 45, 47, 60, 72, 85, 90, 93, 150):
+        n = 16 * tiles
+        got = ad.apply(x[:n], api.AdapterRows(ctx, slots[:n]), y[:n])
+        torch.cuda.synchronize()
+        assert before is None or torch.equal(got[: before.shape[0]], before)
+        before = got
+    check(got, want, off)
 
 
 @pytest.mark.parametrize("shift", [1, 3, 4, 8])
