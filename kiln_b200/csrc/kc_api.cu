@@ -1357,16 +1357,16 @@ void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& o
   if (p->max_len > 16) return;   // a piece of a prompt: partial results of all its chunks would cost what is saved
   // Pieces and chunks that a sequence shares with the one before it; first row; pieces that it does not take itself.
   std::vector<int> pieces(n + 1, 0), common(n + 1, 0), row(n + 1, 0), from(n, 0);
-  int most = 0, any = 0;
+  int most = 0;
   for (int i = 0; i < n; ++i) {
     row[i + 1] = row[i] + seqs[i].len;
     if (i == 0) continue;
     const int limit = std::min(old[i - 1], old[i]) / block_size;
     const int same = (int)(std::mismatch(seqs[i].blocks, seqs[i].blocks + limit, seqs[i - 1].blocks).first - seqs[i].blocks);
-    any = std::max(any, pieces[i] = (int)((long long)same * block_size / ATT_PIECE));
+    pieces[i] = (int)((long long)same * block_size / ATT_PIECE);
     most = std::max(most, common[i] = pieces[i] / per);
   }
-  if (any == 0) return;
+  if (most == 0) return;   // pieces alone would cost whole rows their one launch: 128 sequences behind 369 keys 50 -> 55 us
   // each(first sequence, first row, row behind the last one, last sequence) of the runs of neighbours that `linked` links.
   auto runs = [&](auto&& linked, auto&& each) {
     for (int i = 0, j; i < n; i = j + 1) {

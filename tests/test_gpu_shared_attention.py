@@ -106,10 +106,10 @@ def test_rows_have_the_bits_that_they_have_alone(ctx, heads, kv_heads, dim, name
 
 
 @pytest.mark.parametrize("groups", [
-    [(512, [(1, 512), (1, 600)])], [(0, [(1, 900), (1, 800)])], [(112, [(1, 900 + i) for i in range(200)])], [(2000, [(4, 2040)])], [(0, [(1, 0)])],
+    [(512, [(1, 512), (1, 600)])], [(0, [(1, 900), (1, 800)])], [(496, [(1, 900 + i) for i in range(200)])], [(2000, [(4, 2040)])], [(0, [(1, 0)])],
     [(1024, [(130, 1024)] + [(1, 1200 + i) for i in range(90)])]])
 def test_what_is_not_shared(ctx, groups):
-    """Too little to be read once, less than 128 keys, one sequence, no history, beside a piece of a prompt."""
+    """Too little to be read once, less than a chunk, one sequence, no history, beside a piece of a prompt."""
     seqs, total = tables(groups, 16, 1)
     kv, data = pools(ctx, 4, 128, total, 16, 5)
     q, got, plan = run_both(ctx, kv, data, 16, seqs, 7)
@@ -164,7 +164,7 @@ def test_one_table_for_all(ctx, early):
 
 @pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (28, 4, 128), (32, 8, 64), (16, 8, 256), (64, 8, 128)])
 @pytest.mark.parametrize("rows", [1, 4])
-@pytest.mark.parametrize("prefix", [300, 511, 2048 + 130, 2048 + 400, 4096 + 511])
+@pytest.mark.parametrize("prefix", [512 + 300, 1024 + 511, 2048 + 130, 2048 + 400, 4096 + 511])
 def test_a_prefix_that_ends_inside_a_chunk(ctx, heads, kv_heads, dim, rows, prefix):
     """The pieces of 128 keys that all have of the chunk are taken once, and every sequence goes on from there: in the middle of
     a maximum's life, of a sum and of an output. In two groups, one of single rows."""
