@@ -291,35 +291,37 @@ def test_rows_past_the_shared_ones_are_left(ctx):
     assert (out[0] == 7).all() and (out[91] == 7).all() and torch.equal(out[1:91], api.paged_attention(ctx, kv, 0, q, seqs, 0.125))
 
 
-def test_a_models_steps_share(ctx):
+@pytest.mark.parametrize("n,rows,shared", [(100, 3, 1040), (500, 1, 1408)])     # the second one behind pieces of a chunk too
+def test_a_models_steps_share(ctx, n, rows, shared):
     """A model's verify step over sequences that share a prompt: the logits of a sequence are those it has alone, bit for bit, and
     the K/V it writes too; sampled tokens and counts follow."""
     cfg = PRESETS["tiny-llama-d128"]
-    model = api.CudaModel(ctx, cfg, synth_checkpoint(cfg, seed=1), max_step_tokens=512, max_step_seqs=128)
-    rng, n, shared = np.random.default_rng(1), 100, 1040
-    kv = api.PagedKv(ctx, model.kv_spec(65 + 4 * n + 4, 16))
-    prompt = rng.integers(0, cfg.vocab_size, 1040).tolist()
+    model = api.CudaModel(ctx, cfg, synth_checkpoint(cfg, seed=1), max_step_tokens=512, max_step_seqs=512)
+    rng, first = np.random.default_rng(1), shared // 16
+    kv = api.PagedKv(ctx, model.kv_spec(first + 4 * n + 4, 16))
+    prompt = rng.integers(0, cfg.vocab_size, shared).tolist()
     for at in range(0, shared, 512):
         piece = prompt[at: at + 512]
-        model.forward_step(api.StepBatch(piece, [api.SeqStep(len(piece), at, 0, np.arange(65, dtype=np.uint32))]), kv)
-    own = [np.arange(65 + 4 * i, 69 + 4 * i, dtype=np.uint32) for i in range(n)]
-    ids = rng.integers(0, cfg.vocab_size, (n, 3))
-    seqs = [api.SeqStep(3, shared, 3, np.concatenate([np.arange(65, dtype=np.uint32), own[i]])) for i in range(n)]
+        model.forward_step(api.StepBatch(piece, [api.SeqStep(len(piece), at, 0, np.arange(first, dtype=np.uint32))]), kv)
+    own = [np.arange(first + 4 * i, first + 4 + 4 * i, dtype=np.uint32) for i in range(n)]
+    ids = rng.integers(0, cfg.vocab_size, (n, rows))
+    seqs = [api.SeqStep(rows, shared, rows, np.concatenate([np.arange(first, dtype=np.uint32), own[i]])) for i in range(n)]
     plan = api.AttentionPlan(ctx, kv, cfg.num_attention_heads, seqs)
-    assert shares(plan)
+    read, apart = plan.keys()
+    assert apart - read >= shared // 128 * 128 * n * 0.8
     batch = api.StepBatch(ids.reshape(-1).tolist(), seqs)
     logits = model.forward_step(batch, kv)
     ctx.sync()
     together = logits.clone()
     wrote = kv.read_block_bytes(int(own[7][0]))
-    for i in (0, 7, 50, 99):
-        kv.copy_block(68 + 4 * n - 1, int(own[i][0]))      # what it wrote is written again
+    for i in (0, 7, 50, n - 1):
+        kv.copy_block(first + 4 * n, int(own[i][0]))      # what it wrote is written again
         alone = model.forward_step(api.StepBatch(ids[i].tolist(), [seqs[i]]), kv)
         ctx.sync()
-        assert torch.equal(alone.view(torch.int16), together[3 * i: 3 * i + 3].view(torch.int16))
+        assert torch.equal(alone.view(torch.int16), together[rows * i: rows * (i + 1)].view(torch.int16))
     assert kv.read_block_bytes(int(own[7][0])) == wrote
-    rows, ncom, nacc = model.verify_step(batch, kv)
-    assert torch.equal(torch.from_numpy(rows.astype(np.int64)).cuda(), api.greedy_rows(ctx, together).long())
+    committed, ncom, nacc = model.verify_step(batch, kv)
+    assert torch.equal(torch.from_numpy(committed.astype(np.int64)).cuda(), api.greedy_rows(ctx, together).long())
     assert ctx.device_status() == 0
 
 
