@@ -561,12 +561,17 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
     }
     for (int k = 0; k < rank; ++k) ahead += s.peer_match[k];
   }
-  for (int w = 0; w < warp; ++w) ahead += s.warp_a[w];
-  if (taken <= ahead || taken > ahead + mine) return;
+  // The warp whose vectors have it, and then all threads on those, one each.
+  if (taken <= ahead) return;            // another CTA's
+  int owner = 0;
+  while (owner < DRAW_WARPS && taken > ahead + s.warp_a[owner]) ahead += s.warp_a[owner++];
+  if (owner == DRAW_WARPS) return;
+  const int from = min(v1, v0 + owner * each), to = min(v1, from + each);
   uint32_t left = taken - ahead;                         // of the warp's
-  for (int v = w0; v < w1; v += 32) {
+  for (int first = from; first < to; first += DRAW_THREADS) {
+    const int v = first + tid;
     uint32_t mask = 0;
-    if (v + lane < w1 && matches(x.vec(v + lane), m)) mask = places(m);
+    if (v < to && matches(x.vec(v), m)) mask = places(m);
     const uint32_t own = __popc(mask);
     uint32_t upto = own;
 #pragma unroll
@@ -574,11 +579,18 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
       const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += up;
     }
+    __syncthreads();                     // the last turn's sums have been read
+    if (lane == 31) s.warp_b[warp] = upto;
+    __syncthreads();
+    uint32_t all = 0;
+    for (int w = 0; w < DRAW_WARPS; ++w) {
+      if (w == warp) upto += all;
+      all += s.warp_b[w];
+    }
     if (left <= upto && left > upto - own) {
       for (uint32_t k = left - (upto - own); k > 1; --k) mask &= mask - 1;
-      write((uint32_t)(8 * (v + lane) - x.shift + __ffs(mask) - 1));
+      write((uint32_t)(8 * v - x.shift + __ffs(mask) - 1));
     }
-    const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
     if (left <= all) break;
     left -= all;
   }
