@@ -11,17 +11,17 @@
 // and the order of tokens is the order of values. Counts are whole numbers, so that no order of atomics changes a bit; masses are
 // summed in a fixed tree over the values, whatever the number of CTAs a row has.
 //
-// Counting: a bin a value, of the magnitudes [2^-24, 2^8) of either sign (the home window), 32 KB of shared memory. A row with
+// Counting: a bin a value, of the magnitudes [2^-25, 2^7) of either sign (the home window), 32 KB of shared memory. A row with
 // other magnitudes (but for -inf) takes another pass over itself for each of the eight other windows of 32 binary orders that it has values
 // in, so that any row is exact; zeros are counted apart. The counts and masses of the binades lie in shared memory of every CTA of the row's
 // cluster, which then all look for the same borders. A bin also adds up where its values stand, so that a value that a CTA has once
 // is found without another pass: 512 rows of 256000 159 -> 141 us.
 //
-// What bounds it. Few rows: launch, three cluster barriers and the search's chains of latencies, 2200 cycles a border: one row of 128256 11.6 us,
-// seven of 50001 13.0. Many: the counting, at 0.7 of what shared memory's atomics take (3.6 wavefronts for a warp's 32 places: half of a
+// What bounds it. Few rows: launch, three cluster barriers and the search's chains of latencies, 2200 cycles a border: one row of 128256 11.5 us,
+// seven of 50001 13.1. Many: the counting, at 0.7 of what shared memory's atomics take (3.6 wavefronts for a warp's 32 places: half of a
 // CTA's 37000 cycles at 64128 values), and behind it the accounts and the search, which only the SM's other CTA can fill: 128 rows
-// of 128256 31 us, 192 41 (384 CTAs in 296 places, 7.5 us at a copy's rate), 512 of 256000 140 (40). Three CTAs an SM of 256 to 384 threads:
-// 40 to 44 and 153 to 162; one CTA a row 47 at 192.
+// of 128256 30 us, 192 37 (384 CTAs in 296 places, 7.5 us at a copy's rate; 8 more where one of the rows has a value outside the home window),
+// 512 of 256000 139 (40). Three CTAs an SM of 256 to 384 threads 40 to 44 and 153 to 162 where this was 41 and 141; one CTA a row 47 at 192.
 #include "kc_fused.cuh"
 #include "kc_umma.cuh"
 
@@ -34,8 +34,8 @@ namespace {
 constexpr int draw_threads(int ctas) { return ctas > 2 ? 256 : 512; }
 constexpr int DRAW_WINDOW = 4096;                 // magnitudes (bf16 without the sign) of a window, 32 binades
 constexpr int DRAW_LOW = 4, DRAW_SIDE = 4128;     // of a sign's bins: the window's first one; all of them (next to the window's: what lies below, above)
-constexpr int DRAW_HOME = 4;                      // the window that holds a language model's logits: magnitudes 2^-24 to 2^8
-constexpr int DRAW_BASE0 = 103 * 128 - DRAW_HOME * DRAW_WINDOW;   // first magnitude of window 0 (below zero: it is a short one)
+constexpr int DRAW_HOME = 4;                      // the window that holds a language model's logits: magnitudes 2^-25 to 2^7
+constexpr int DRAW_BASE0 = 102 * 128 - DRAW_HOME * DRAW_WINDOW;   // first magnitude of window 0 (below zero: it is a short one)
 constexpr int DRAW_WINDOWS = 9;
 // A bin counts in its low bits and adds up the indices of the vectors in the high ones, which is the place of a value that occurs once.
 constexpr int DRAW_AT = 18;
@@ -615,7 +615,7 @@ cudaError_t launch_draw_rows(const bf16* logits, long long ld, int rows, int voc
                              int skip_greedy) {
   if (rows <= 0) return cudaSuccess;
   // As many CTAs a row as the SMs hold at once, two on each, and two where the rows are more. Rows of 128256 with 2, 4 and 8
-  // CTAs each: one row 17.6, 13.9 and 11.6 us; 192 rows 40.8, 49.2 and 94.7.
+  // CTAs each: one row 17.6, 13.9 and 11.6 us; 192 rows 37.4, 49.2 and 94.7.
   const int room = 2 * sm_count / rows;
   auto as = room >= 8 ? draw_as<8> : room >= 4 ? draw_as<4> : draw_as<2>;
   return as(logits, ld, rows, vocab, settings, uniform, tokens, logprobs, s, tokens_host, logprobs_host, skip_greedy);
