@@ -12,8 +12,8 @@
 // summed in a fixed tree over the values, whatever the number of CTAs a row has.
 //
 // Counting: a bin a value, of the magnitudes [2^-25, 2^7) of either sign (the home window), 32 KB of shared memory. A row with
-// other magnitudes (but for -inf) takes another pass over itself for each of the eight other windows of 32 binary orders that it has values
-// in, so that any row is exact; zeros are counted apart. The counts and masses of the binades lie in shared memory of every CTA of the row's
+// other magnitudes (but for -inf, and one smaller value of either sign, as a row in five hundred has) takes another pass over itself for each
+// of the eight other windows of 32 binary orders that it has values in, so that any row is exact; zeros are counted apart. The counts and masses of the binades lie in shared memory of every CTA of the row's
 // cluster, which then all look for the same borders. A bin also adds up where its values stand, so that a value that a CTA has once
 // is found without another pass: 512 rows of 256000 159 -> 141 us.
 //
@@ -55,7 +55,7 @@ struct DrawShared {
   uint4 lane_counts[64 / C][32];                  // how often each value occurs in the row, in falling order
   double mass[DRAW_RUNS][32];                     // of a binade; later of its run up to it
   uint32_t count[DRAW_RUNS][32];
-  uint32_t peer_top[8], peer_seen[8], peer_zeros[8], peer_match[8];   // what each CTA of the cluster found
+  uint32_t peer_top[8], peer_out[8], peer_lone[8], peer_seen[8], peer_zeros[8], peer_match[8];   // what each CTA of the cluster found
   uint32_t warp_a[draw_threads(C) / 32], warp_b[draw_threads(C) / 32];
   uint32_t far;                                   // whether a finite value lies below the window's negative ones
   uint32_t above;                                 // tokens of w >= min_p, over the cluster
@@ -200,6 +200,8 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
   const uint32_t at_step = places_fit ? 1u << DRAW_AT : 0u, count_mask = places_fit ? (1u << DRAW_AT) - 1 : ~0u;
   static_assert(8 << (32 - DRAW_AT) < 1 << DRAW_AT, "counts");
 
+  const bool lone_places = vocab <= 262000;   // whatever the cluster's size: a row's bits do not hang on it
+  static_assert((262000 + 14) / 8 / 2 + 1 <= 1 << (32 - DRAW_AT), "places");
   // ---- pass over the row: bins of the home window, and the maximum. Two values at a time as halves of a register: their
   // magnitudes, held between the window's neighbours on either side, become places of bins by whole-number arithmetic that
   // neither half carries out of ----
@@ -231,10 +233,43 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
   }
   __syncthreads();
   const float m_cta = warp_max(__uint_as_float(s.warp_a[lane & (DRAW_WARPS - 1)]));
-  // Values outside the home window (NaN among them, masked ones not): zeros are counted, of the others what windows they are in.
-  uint32_t seen = 0, zeros = 0;
+  // Values outside the home window, masked ones apart: how many lie below it (zeros and NaN among them; 2: more than one) of either sign,
+  // whether any lies above. In a vocabulary's normal rows there is one below now and then, which its bin's place finds.
   constexpr int HIGH = DRAW_LOW + DRAW_WINDOW;
-  if (!greedy && (s.bins[DRAW_LOW - 1] | s.bins[HIGH] | s.bins[DRAW_SIDE + DRAW_LOW - 1] | s.far)) {
+  if (tid < C) {
+    uint32_t out = (s.bins[HIGH] | s.far) ? 16u : 0u, lone = 0;
+#pragma unroll
+    for (int sign = 0; sign < 2; ++sign) {
+      const uint32_t bin = s.bins[sign * DRAW_SIDE + DRAW_LOW - 1], n = min(bin & count_mask, 2u);
+      out |= n << (2 * sign);
+      if (n == 1 && lone_places) {
+        const uint4 u = x.vec(v0 + (int)(bin >> DRAW_AT));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = (w[j >> 1] >> (16 * (j & 1))) & 0xFFFFu, mag = b & 0x7FFFu;
+          if ((int)(b >> 15) == sign && (mag < FIRST || mag > BF16_INF)) lone |= mag << (16 * sign);
+        }
+      }
+    }
+    peer_put(&s.peer_top[rank], tid, __float_as_uint(m_cta));
+    peer_put(&s.peer_out[rank], tid, out);
+    peer_put(&s.peer_lone[rank], tid, lone);
+  }
+  cluster_sync();
+  float largest = -INFINITY;
+  uint32_t seen = 0, zeros = 0, lone = 0, above_window = 0, below[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    largest = fmaxf(largest, __uint_as_float(s.peer_top[k]));
+    const uint32_t out = s.peer_out[k];
+    above_window |= out >> 4; below[0] += out & 3; below[1] += out >> 2 & 3;
+    lone |= s.peer_lone[k];
+  }
+  // From here on every branch that holds a barrier is taken by the whole cluster: what it hangs on is the same in all its CTAs.
+  if (above_window || max(below[0], below[1]) > (lone_places ? 1u : 0u)) {
+    // A pass over the row: zeros are counted, of the others what windows they are in.
+    below[0] = below[1] = 0;
     x.each<DRAW_THREADS>(v0, v1, tid, [&](const uint4& u, int) {
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -246,25 +281,22 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
     });
     seen = __reduce_or_sync(0xffffffffu, seen) & ~(1u << DRAW_HOME);
     zeros = __reduce_add_sync(0xffffffffu, zeros);
-    __syncthreads();                     // the warps' maxima have been read
-    if (lane == 0) { s.warp_a[warp] = seen; s.warp_b[warp] = zeros; }
+    if (lane == 0) { s.warp_a[warp] = seen; s.warp_b[warp] = zeros; }   // the warps' maxima have been read
     __syncthreads();
     seen = zeros = 0;
-    if (tid < C)
+    if (tid < C) {
       for (int w = 0; w < DRAW_WARPS; ++w) { seen |= s.warp_a[w]; zeros += s.warp_b[w]; }
-  }
-  if (tid < C) {
-    peer_put(&s.peer_top[rank], tid, __float_as_uint(m_cta));
-    peer_put(&s.peer_seen[rank], tid, seen);
-    peer_put(&s.peer_zeros[rank], tid, zeros);
-  }
-  cluster_sync();
-  float largest = -INFINITY;
-  seen = zeros = 0;
+      peer_put(&s.peer_seen[rank], tid, seen);
+      peer_put(&s.peer_zeros[rank], tid, zeros);
+    }
+    cluster_sync();
+    seen = zeros = 0;
 #pragma unroll
-  for (int k = 0; k < C; ++k) { largest = fmaxf(largest, __uint_as_float(s.peer_top[k])); seen |= s.peer_seen[k]; zeros += s.peer_zeros[k]; }
+    for (int k = 0; k < C; ++k) { seen |= s.peer_seen[k]; zeros += s.peer_zeros[k]; }
+  } else {
+    zeros = (below[0] && (lone & 0xFFFFu) == 0) + (below[1] && lone >> 16 == 0);
+  }
   largest += 0.f;                        // -0 is +0
-  // From here on every branch that holds a barrier is taken by the whole cluster: what it hangs on is the same in all its CTAs.
   const bool empty = largest == -INFINITY;   // nothing but masked tokens and NaN: token 0
   uint32_t bits = __float_as_uint(largest) >> 16, taken = 1;
   int resident = DRAW_HOME;              // window of the bins
@@ -365,6 +397,15 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
       const double w = weight_of(0);
       s.count[DRAW_ZERO][0] = zeros; s.mass[DRAW_ZERO][0] = zeros * w;
       if (w >= min_p) peer_add(&s.above, rank, zeros);   // every CTA for itself
+    }
+    if (tid < 2 && below[tid]) {           // the one value below the window, positive or negative: the only one of its run
+      const uint32_t mag = lone >> (16 * tid) & 0xFFFFu, at = mag - (uint32_t)DRAW_BASE0;
+      if (mag != 0 && mag < BF16_INF) {
+        const int run = tid ? DRAW_ZERO + 1 + (int)(at / DRAW_WINDOW) : DRAW_ZERO - 1 - (int)(at / DRAW_WINDOW), k = at % DRAW_WINDOW / 128;
+        const double w = weight_of(tid << 15 | mag);
+        s.count[run][tid ? k : 31 - k] = 1; s.mass[run][tid ? k : 31 - k] = w;
+        if (w >= min_p) peer_add(&s.above, rank, 1u);
+      }
     }
     for (int w = 0; w < DRAW_WINDOWS; ++w)
       if (seen >> w & 1) enter(w, true);

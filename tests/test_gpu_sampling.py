@@ -161,6 +161,26 @@ def test_rows_do_not_hang_on_their_number(ctx):
         assert torch.equal(got, want[:n]) and torch.equal(q.view(torch.int32), p[:n].view(torch.int32))
 
 
+@pytest.mark.parametrize("rows", [1, 40, 80, 200])
+@pytest.mark.parametrize("vocab", [9, 300, 5003, 128256])
+def test_values_below_all_others(ctx, rows, vocab):
+    """One value of a magnitude far below the rest's, of either sign or both, a zero or NaN as it may be, or two: in the middle of a row,
+    at its end, as its largest."""
+    rng = np.random.default_rng(rows + vocab)
+    tiny = [2.0 ** -26, -2.0 ** -26, 1e-30, -1e-30, 0.0, -0.0, math.nan, 1e-40, -1e-40, 2.0 ** -25 * 0.99]
+    x = language(rows, vocab, 17)
+    host = x.float().cpu()
+    host[::3] = -host[::3].abs() - 0.5                   # below zero: a tiny value is the largest
+    for r in range(rows):
+        places = rng.choice(vocab, 3, replace=False)
+        if r % 4 == 3:
+            places[0] = vocab - 1
+        for k in range([1, 1, 2, 1, 3][r % 5]):
+            host[r, places[k]] = tiny[(r // 2 + 3 * k) % len(tiny)]
+    settings = [(float(rng.choice([0.7, 1.0, 100.0])), int(rng.choice([0, 1, 2, 40])), float(rng.choice([1.0, 0.5, 0.95])), float(rng.choice([0.0, 0.3, 1.0]))) for _ in range(rows)]
+    check(ctx, host.to(torch.bfloat16).cuda(), settings, rng.choice([0.0, 0.3, 0.999, 1 - 2 ** -24], rows).astype(np.float32).tolist())
+
+
 @pytest.mark.parametrize("rows,vocab", [(160, 270001), (80, 530003), (1, 1048569), (1, 1200000)])
 def test_long_rows(ctx, rows, vocab):
     """More values than a bin has room to say where they stand (8 to the vector, 16384 vectors a CTA), and just as many."""
