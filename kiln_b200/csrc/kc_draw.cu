@@ -17,11 +17,10 @@
 // cluster, which then all look for the same borders. A bin also adds up where its values stand, so that a value that a CTA has once
 // is found without another pass: 512 rows of 256000 159 -> 141 us.
 //
-// What bounds it. Few rows: launch, three cluster barriers and the search's chains of latencies, 2200 cycles a border: one row of 128256 11.5 us,
-// seven of 50001 13.1. Many: the counting, at 0.7 of what shared memory's atomics take (3.6 wavefronts for a warp's 32 places: half of a
-// CTA's 37000 cycles at 64128 values), and behind it the accounts and the search, which only the SM's other CTA can fill: 128 rows
-// of 128256 30 us, 192 37 (384 CTAs in 296 places, 7.5 us at a copy's rate; 8 more where one of the rows has a value outside the home window),
-// 512 of 256000 139 (40). Three CTAs an SM of 256 to 384 threads 40 to 44 and 153 to 162 where this was 41 and 141; one CTA a row 47 at 192.
+// What bounds it. Few rows: launch, three cluster barriers and the search's chains of latencies, 2200 cycles a border: one row of 128256 11.6 us,
+// seven of 50001 13.1. Many: the counting, at 0.7 of what shared memory's atomics take (3.6 wavefronts for a warp's 32 places), and
+// behind it the accounts and the search, 17000 cycles that only the SM's other CTAs can fill: 128 rows of 128256 24.5 us, 192 31.9 (384 CTAs
+// in 444 places; 7.5 us at a copy's rate), 512 of 256000 102 (40). One CTA a row 47 at 192.
 #include "kc_fused.cuh"
 #include "kc_umma.cuh"
 
@@ -29,9 +28,9 @@ namespace kc {
 
 namespace {
 
-// Threads of a CTA: half as many where a row has many CTAs, whose barriers then take less (one row of 128256 12.8 -> 11.5 us; with two CTAs a row
-// 512 rows of 256000 141 -> 159 us).
-constexpr int draw_threads(int ctas) { return ctas > 2 ? 256 : 512; }
+// Threads of a CTA, by the CTAs of a row and of an SM: half as many where a row has many, whose barriers then take less (one row of 128256 12.8 ->
+// 11.5 us), and where an SM has three.
+constexpr int draw_threads(int ctas, int resident) { return ctas > 2 || resident > 2 ? 256 : 512; }
 constexpr int DRAW_WINDOW = 4096;                 // magnitudes (bf16 without the sign) of a window, 32 binades
 constexpr int DRAW_LOW = 4, DRAW_SIDE = 4128;     // of a sign's bins: the window's first one; all of them (next to the window's: what lies below, above)
 constexpr int DRAW_HOME = 4;                      // the window that holds a language model's logits: magnitudes 2^-25 to 2^7
@@ -46,17 +45,17 @@ constexpr uint32_t BF16_INF = 0x7F80u;
 static_assert(DRAW_BASE0 % 128 == 0 && DRAW_BASE0 + DRAW_WINDOWS * DRAW_WINDOW > 0x7F80, "windows cover all magnitudes in whole binades");
 
 // C: CTAs of a row's cluster. Every C-th binade of the resident window is a CTA's own, to add up over the cluster's parts of the row.
-template <int C>
+template <int C, int RESIDENT>
 struct DrawShared {
   uint32_t bins[2 * DRAW_SIDE];                   // [sign][magnitude]: how often the value occurs in this CTA's part of the row, and where (DRAW_AT)
   double lane_weight[64 / C][32];                 // own binades, four values a lane: the weight of the lane's first one,
   double lane_mass[64 / C][32];                   // mass and
   uint32_t lane_count[64 / C][32];                // tokens of the binade up to the lane's last one
-  uint4 lane_counts[64 / C][32];                  // how often each value occurs in the row, in falling order
+  uint4 lane_counts[C > 2 ? 64 / C : 1][32];      // C > 2: how often each value occurs in the row, in falling order
   double mass[DRAW_RUNS][32];                     // of a binade; later of its run up to it
   uint32_t count[DRAW_RUNS][32];
   uint32_t peer_top[8], peer_out[8], peer_lone[8], peer_seen[8], peer_zeros[8], peer_match[8];   // what each CTA of the cluster found
-  uint32_t warp_a[draw_threads(C) / 32], warp_b[draw_threads(C) / 32];
+  uint32_t warp_a[draw_threads(C, RESIDENT) / 32], warp_b[draw_threads(C, RESIDENT) / 32];
   uint32_t far;                                   // whether a finite value lies below the window's negative ones
   uint32_t above;                                 // tokens of w >= min_p, over the cluster
   double ratio[32];                               // of the weights of neighbouring values, by binade of the resident window
@@ -160,14 +159,14 @@ struct DrawRow {
   }
 };
 
-template <int C>
-__global__ void __launch_bounds__(draw_threads(C), 2)
+template <int C, int RESIDENT>
+__global__ void __launch_bounds__(draw_threads(C, RESIDENT), RESIDENT)
 draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const DrawSetting* __restrict__ settings,
                  const float* __restrict__ uniform, uint32_t* __restrict__ tokens, float* __restrict__ logprobs,
                  uint32_t* __restrict__ tokens_host, float* __restrict__ logprobs_host, int skip_greedy) {
-  constexpr int DRAW_THREADS = draw_threads(C), DRAW_WARPS = DRAW_THREADS / 32;
+  constexpr int DRAW_THREADS = draw_threads(C, RESIDENT), DRAW_WARPS = DRAW_THREADS / 32;
   extern __shared__ __align__(16) uint8_t draw_smem[];
-  DrawShared<C>& s = *reinterpret_cast<DrawShared<C>*>(draw_smem);
+  DrawShared<C, RESIDENT>& s = *reinterpret_cast<DrawShared<C, RESIDENT>*>(draw_smem);
   pdl_launch_dependents();
   cluster_arrive();                      // waited for before the first access to another CTA's shared memory: it has started by then
   const int row_index = blockIdx.x / C, rank = blockIdx.x % C;
@@ -362,7 +361,8 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
           const double mu = __shfl_up_sync(0xffffffffu, m, o);
           if (lane >= o) { n += nu; m += mu; }
         }
-        s.lane_counts[k / C][lane] = v; s.lane_weight[k / C][lane] = first; s.lane_mass[k / C][lane] = m; s.lane_count[k / C][lane] = n;
+        if (C > 2) s.lane_counts[k / C][lane] = v;
+        s.lane_weight[k / C][lane] = first; s.lane_mass[k / C][lane] = m; s.lane_count[k / C][lane] = n;
         if (!enters) continue;
         above = __reduce_add_sync(0xffffffffu, above);
         n = __shfl_sync(0xffffffffu, n, 31); m = __shfl_sync(0xffffffffu, m, 31);
@@ -471,7 +471,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
         ln = peer_get(&s.lane_count[k / C][lane], owner);
         lm = peer_get(&s.lane_mass[k / C][lane], owner);
         const double lw = peer_get(&s.lane_weight[k / C][lane], owner);
-        const uint4 v = peer_get4(&s.lane_counts[k / C][lane].x, owner);
+        const uint4 v = C > 2 ? peer_get4(&s.lane_counts[k / C][lane].x, owner) : in_order(k, counts(k));
         const int who = first_of((v.x | v.y | v.z | v.w) && crossed(what, cn + ln, cm + lm, want, target), (v.x | v.y | v.z | v.w) != 0);
         cn += ahead_of(ln, who); cm += mass_ahead_of(lm, who);
         c[0] = __shfl_sync(0xffffffffu, v.x, who); c[1] = __shfl_sync(0xffffffffu, v.y, who);
@@ -637,15 +637,15 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
   }
 }
 
-template <int C>
+template <int C, int RESIDENT>
 cudaError_t draw_as(const bf16* logits, long long ld, int rows, int vocab, const DrawSetting* settings, const float* uniform, uint32_t* tokens,
                     float* logprobs, cudaStream_t s, uint32_t* tokens_host, float* logprobs_host, int skip_greedy) {
   static DeviceOnce configured;   // the attribute belongs to the device's copy of the kernel
   if (configured.first_on_current_device()) {
-    cudaError_t e = cudaFuncSetAttribute(draw_rows_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DrawShared<C>));
+    cudaError_t e = cudaFuncSetAttribute(draw_rows_kernel<C, RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DrawShared<C, RESIDENT>));
     if (e != cudaSuccess) { configured.forget_current_device(); return e; }
   }
-  return launch_k_cluster(C, draw_rows_kernel<C>, dim3(rows * C), dim3(draw_threads(C)), sizeof(DrawShared<C>), s, logits, ld, vocab, settings, uniform,
+  return launch_k_cluster(C, draw_rows_kernel<C, RESIDENT>, dim3(rows * C), dim3(draw_threads(C, RESIDENT)), sizeof(DrawShared<C, RESIDENT>), s, logits, ld, vocab, settings, uniform,
                           tokens, logprobs, tokens_host, logprobs_host, skip_greedy);
 }
 
@@ -655,10 +655,11 @@ cudaError_t launch_draw_rows(const bf16* logits, long long ld, int rows, int voc
                              uint32_t* tokens, float* logprobs, int sm_count, cudaStream_t s, uint32_t* tokens_host, float* logprobs_host,
                              int skip_greedy) {
   if (rows <= 0) return cudaSuccess;
-  // As many CTAs a row as the SMs hold at once, two on each, and two where the rows are more. Rows of 128256 with 2, 4 and 8
-  // CTAs each: one row 17.6, 13.9 and 11.6 us; 192 rows 37.4, 49.2 and 94.7.
+  // As many CTAs a row as the SMs hold at once, two on each, and two where the rows are more: then three CTAs an SM. Rows of 128256 with 2, 4 and
+  // 8 CTAs each: one row 17.6, 13.9 and 11.5 us; 192 rows 36.7, 49 and 95. Two and three CTAs an SM: 128 rows 24.5 and 26.4, 192 36.7 and 31.7, 300
+  // of 50001 39.6 and 34.2, 512 of 256000 107 and 102.
   const int room = 2 * sm_count / rows;
-  auto as = room >= 8 ? draw_as<8> : room >= 4 ? draw_as<4> : draw_as<2>;
+  auto as = room >= 8 ? draw_as<8, 2> : room >= 4 ? draw_as<4, 2> : room >= 2 ? draw_as<2, 2> : draw_as<2, 3>;
   return as(logits, ld, rows, vocab, settings, uniform, tokens, logprobs, s, tokens_host, logprobs_host, skip_greedy);
 }
 
