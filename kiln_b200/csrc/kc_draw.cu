@@ -429,8 +429,10 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
     enum { COUNT, REACH, EXCEED };
     uint32_t n_run = 0, n = 0;           // of the runs up to this lane's; tokens kept so far
     double m_run = 0.0, mass = 0.0;      // their masses
+    bool has_tokens = false;             // this lane's run
     if (warp == 0) {
       if (lane < DRAW_RUNS) { n_run = s.count[lane][31]; m_run = s.mass[lane][31]; }
+      has_tokens = n_run != 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t nu = __shfl_up_sync(0xffffffffu, n_run, o);
@@ -442,8 +444,9 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
     struct { uint32_t bits, taken, n; double mass, weight; } at = {0, 0, 0, 0.0, 0.0};   // value, how many of it, tokens and mass up to there
     auto crossed = [](int what, uint32_t count, double m, uint32_t want, double target) { return what == COUNT ? count >= want : what == REACH ? m >= target : m > target; };
     // The border that a number of tokens (COUNT) or a mass reaches (REACH) or exceeds (EXCEED): in `at` with -1 returned, or
-    // the window that has to be resident; -2 where nothing reaches it. Run, binade, lane, value: of each the first one at whose
-    // end the border is crossed; a sum may be a rounding apart from its parts', and then the last part has the border.
+    // the window that has to be resident; -2 where nothing reaches it. Run, binade, lane, value: of each the first one with tokens at
+    // whose end the border is crossed: the tree adds up each end's masses in an order of its own, so that the sum at the end of an empty part may be
+    // a rounding above its neighbours'. A sum may be a rounding apart from its parts' too, and then the last part has the border.
     auto border = [&](int what, uint32_t want, double target) -> int {
       auto first_of = [&](bool holds, bool there) {
         const uint32_t h = __ballot_sync(0xffffffffu, holds), t = __ballot_sync(0xffffffffu, there);
@@ -451,7 +454,7 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
       };
       auto ahead_of = [&](uint32_t v, int i) { const uint32_t u = __shfl_sync(0xffffffffu, v, (i + 31) & 31); return i ? u : 0u; };
       auto mass_ahead_of = [&](double v, int i) { const double u = __shfl_sync(0xffffffffu, v, (i + 31) & 31); return i ? u : 0.0; };
-      const uint32_t runs = __ballot_sync(0xffffffffu, crossed(what, n_run, m_run, want, target));
+      const uint32_t runs = __ballot_sync(0xffffffffu, has_tokens && crossed(what, n_run, m_run, want, target));
       if (!runs) return -2;
       const int run = __ffs(runs) - 1;
       uint32_t cn = ahead_of(n_run, run), c[4] = {0, 0, 0, 0};   // tokens and mass ahead of what has been narrowed down to
@@ -522,8 +525,9 @@ draw_rows_kernel(const bf16* __restrict__ logits, long long ld, int vocab, const
             want = max(s.above, 1u);
             if (!(set.min_p > 0.f && want < n)) continue;
           } else if (stage == 3) {
+            if (!(unit < 1.0)) continue; // 1 and more, NaN: a rounding of a sum is not to decide
             what = EXCEED; target = unit * mass;
-          } else {                       // u of 1 and more, NaN: the last one kept
+          } else {                       // the last one kept, also where no sum exceeds the target
             want = n;
           }
           window = border(what, want, target);
