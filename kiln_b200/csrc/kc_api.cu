@@ -368,6 +368,12 @@ static int capturing(kc_ctx* c, bool* is) {
   *is = st != cudaStreamCaptureStatusNone;
   return KC_OK;
 }
+// Copies and allocations of a handle's own are no part of a graph.
+static int not_captured(kc_ctx* c, const char* where) {
+  bool is = false;
+  RC(capturing(c, &is));
+  return is ? fail(KC_ERR_INVALID, "%s: the context's stream is being captured", where) : KC_OK;
+}
 // A launch bracketed by the profile's events has no time of its own inside a graph.
 static int not_profiled_in_graph(kc_ctx* c, const char* where) {
   bool is = false;
@@ -745,6 +751,7 @@ extern "C" int kc_adapters_create(kc_ctx_t c, int32_t in_features, int32_t out_f
   if (max_rank > LORA_MAX_RANK) return fail(KC_ERR_UNSUPPORTED, "kc_adapters_create: rank %d (at most %d)", max_rank, LORA_MAX_RANK);
   OnDevice on;
   CK(on.enter(c->device));
+  RC(not_captured(c, "kc_adapters_create"));
   kc_adapters* ad = new kc_adapters;
   ad->ctx = c; ad->device = c->device; ad->n_in = in_features; ad->n_out = out_features; ad->slots = slots; ad->max_rank = max_rank;
   ad->stride = lora_stride(max_rank);
@@ -777,6 +784,7 @@ extern "C" int kc_adapters_set(kc_adapters_t ad, int32_t slot, const void* a, co
   kc_ctx* c = ad->ctx;
   OnDevice on;
   CK(on.enter(ad->device));
+  RC(not_captured(c, "kc_adapters_set"));
   const LoraSlot meta{rank, scale};
   if (rank > 0) {
     const size_t a_slot = (size_t)ad->stride * ad->n_in, b_slot = (size_t)ad->stride * ad->n_out;
@@ -803,6 +811,7 @@ extern "C" int kc_adapter_rows_create(kc_ctx_t c, const int32_t* slot_of_row, in
   }
   OnDevice on;
   CK(on.enter(c->device));
+  RC(not_captured(c, "kc_adapter_rows_create"));
   std::vector<int32_t> order;
   std::vector<LoraTile> tiles;
   try {
@@ -2185,9 +2194,7 @@ static int set_attn_plan(kc_attn_plan* p, const kc_seq_step* seqs, int32_t n_seq
   long long n = 0;
   for (int i = 0; i < n_seqs; ++i) n += std::max(0, seqs[i].len);
   if (n_seqs < 1 || n < 1 || n > 1 << 24) return fail(KC_ERR_INVALID, "%s: %lld token(s) of %d sequence(s)", where, n, n_seqs);
-  bool busy = false;
-  RC(capturing(p->ctx, &busy));
-  if (busy) return fail(KC_ERR_INVALID, "%s: the context's stream is being captured", where);
+  RC(not_captured(p->ctx, where));
   std::vector<uint32_t> ids((size_t)n, 0);
   if (!p->shell[0]) RC(new_shell(p->ctx, &p->shell[0]));
   set_shell(p->shell[0], p->kv, p->num_heads, (int)n, n_seqs);

@@ -153,3 +153,32 @@ for h in (past, who): lib.kc_adapter_rows_free(h)
 lib.kc_adapters_free(bank); lib.kc_adapters_free(None); lib.kc_adapter_rows_free(None)
 assert lib.kc_live_objects() == before
 """)
+
+
+def test_adapters_are_made_and_set_outside_captures(graphs):
+    """Inside one the fill that empties a new bank's slots and the copies into one would be the graph's, not the call's."""
+    run(graphs, """
+bank, who = C.c_void_p(), C.c_void_p()
+slots = (C.c_int32 * 3)(0, -1, 1)
+def make():
+    b, r = C.c_void_p(), C.c_void_p()
+    return lib.kc_adapters_create(ctx, 64, 48, 3, 20, C.byref(b)), lib.kc_adapter_rows_create(ctx, slots, 3, C.byref(r)), b, r
+rc, rc_rows, bank, who = make()
+ok(rc); ok(rc_rows)
+def put():
+    return lib.kc_adapters_set(bank, 1, at, at, 20, 1.0, 0), lib.kc_adapters_set(bank, 1, None, None, 0, 0.0, 0)
+before = lib.kc_live_objects()
+fake.fake_reset()
+fake.fake_capture(1)
+assert put() == (L.KC_ERR_INVALID, L.KC_ERR_INVALID) and b"captured" in lib.kc_last_error()
+rc, rc_rows, b, r = make()
+assert rc == rc_rows == L.KC_ERR_INVALID and not b.value and not r.value and lib.kc_live_objects() == before
+assert not calls()
+ok(lib.kc_adapters_apply(bank, who, at, at + 4096, at + 4096))     # the product may be captured
+fake.fake_capture(0)
+assert put() == (0, 0)
+rc, rc_rows, b, r = make()
+ok(rc); ok(rc_rows)
+for h in (r, who): lib.kc_adapter_rows_free(h)
+for h in (b, bank): lib.kc_adapters_free(h)
+""")
