@@ -402,8 +402,10 @@ KC_API int64_t kc_static_scratch_bytes(void);
  * result is rounded to bf16.
  * kc_adapters_create makes the adapters of one projection: `slots` of them, of ranks up to max_rank (1..128), empty to begin with; in_features a
  * multiple of 32. kc_adapters_set copies A bf16 [rank, in] and B bf16 [out, rank] into a slot, in place of what it held
- * (rank 0 empties it; a and b may then be NULL); it returns when the copies are done, behind everything queued before it. Both, and
- * kc_adapter_rows_create, are refused while the context's stream is being captured. */
+ * (rank 0 empties it; a and b may then be NULL); it returns when the copies are done, behind everything that the context's stream
+ * holds. Graphs that are replayed on another stream are the caller's to order (kc_ctx_wait_stream ahead of it), and
+ * need their adapters and rows until the last replay is done. kc_adapters_create, kc_adapters_set and kc_adapter_rows_create
+ * are refused while the context's stream is being captured. */
 typedef struct kc_adapters* kc_adapters_t;
 typedef struct kc_adapter_rows* kc_adapter_rows_t;
 KC_API int kc_adapters_create(kc_ctx_t ctx, int32_t in_features, int32_t out_features, int32_t slots, int32_t max_rank,

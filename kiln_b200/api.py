@@ -255,9 +255,9 @@ class Context:
         return int(L.lib().kc_ctx_stream(self._h) or 0)
 
     def on_current_stream(self, call, *args) -> None:
-        """``call(*args)``, an entry point that does not synchronise, as part of torch's current stream of this
-        context's device: behind what that stream and the context's hold, and ahead of what either is given later. The host
-        waits for nothing, also in a capture into a graph. A program that makes the context's stream torch's current one
+        """``call(*args)``, work on the context's stream, as part of torch's current stream of this context's device: behind
+        what that stream and the context's hold, and ahead of what either is given later. The host waits for nothing but what
+        the entry point itself waits for, also in a capture into a graph. A program that makes the context's stream torch's current one
         (``torch.cuda.ExternalStream(ctx.stream)``) spares the two events that this takes."""
         current = _raw_stream(self.device)
         if current == self._stream:
@@ -656,20 +656,19 @@ class Adapters:
         ctx._adopt(self)
 
     def set(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
-        """Copies A bf16 [rank, in] and B bf16 [out, rank], on the host or this device, into the slot."""
+        """Copies A bf16 [rank, in] and B bf16 [out, rank], on the host or this device, into the slot: behind what the context's
+        stream and torch's current one hold, graphs replayed there among it. Returns when it is done; refused in a capture."""
         rank = a.shape[0]
         if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16 or a.shape != (rank, self.in_features) or b.shape != (self.out_features, rank) or a.is_cuda != b.is_cuda:
             raise ValueError(f"A bf16 [rank, {self.in_features}] and B bf16 [{self.out_features}, rank] on one device")
         if a.is_cuda and (a.device.index != self.ctx.device or b.device.index != self.ctx.device):
             raise ValueError(f"tensors of a context on cuda:{self.ctx.device}")
         a, b = a.contiguous(), b.contiguous()
-        if a.is_cuda:
-            torch.cuda.current_stream(a.device).synchronize()
-        check(L.lib().kc_adapters_set(self._h, slot, a.data_ptr(), b.data_ptr(), rank, scale, int(a.is_cuda)))
+        self.ctx.on_current_stream(L.lib().kc_adapters_set, self._h, slot, a.data_ptr(), b.data_ptr(), rank, scale, int(a.is_cuda))
 
     def clear(self, slot: int) -> None:
-        """Empties the slot: rows that use it keep their y."""
-        check(L.lib().kc_adapters_set(self._h, slot, None, None, 0, 0.0, 0))
+        """Empties the slot: rows that use it keep their y. In the order of ``set``."""
+        self.ctx.on_current_stream(L.lib().kc_adapters_set, self._h, slot, None, None, 0, 0.0, 0)
 
     def apply(self, x: torch.Tensor, rows: AdapterRows, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """y + scale B (A x), row by row: x bf16 [m, in], y bf16 [m, out] (a projection's output), ``out`` for the result (y itself: in

@@ -215,6 +215,56 @@ def test_streams_and_graphs(ctx):
     ctx.sync()
 
 
+def test_a_slot_is_set_behind_a_graph_in_flight(ctx):
+    """A replay on another stream than the context's, still to run when the host sets or empties the slot, has the slot as it was."""
+    ad, parts = bank(ctx, 256, 512, [16, 16], 3)
+    _, others = bank(ctx, 256, 512, [16, 16], 4)
+    rows = api.AdapterRows(ctx, [0, 1, 1, -1, 0])
+    x, y = inputs(5, 256, 512, 1)
+    first = ad.apply(x, rows, y)
+    out = torch.empty_like(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ad.apply(x, rows, y, out=out)
+    stream = torch.cuda.Stream()
+    on_host = [t.to(torch.bfloat16).cpu() for t in others[0][:2]]
+    changes = [lambda: ad.set(0, *on_host), lambda: ad.set(0, *(t.cuda() for t in on_host)), lambda: ad.clear(0)]
+    for change in changes:
+        ad.set(0, *(t.to(torch.bfloat16) for t in parts[0][:2]), parts[0][2])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            out.zero_()
+            torch.cuda._sleep(100_000_000)                         # some 50 ms
+            graph.replay()
+            change()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not torch.equal(out, first)
+        assert torch.equal(out, ad.apply(x, rows, y))
+
+
+def test_a_slot_is_not_set_in_a_capture(ctx):
+    """Refused, and the capture is what it would be without."""
+    ad, parts = bank(ctx, 256, 512, [16, 16], 3)
+    rows = api.AdapterRows(ctx, [0, 1, 1, -1, 0])
+    x, y = inputs(5, 256, 512, 1)
+    want, out = ad.apply(x, rows, y), torch.empty_like(y)
+    a, b = (t.to(torch.bfloat16).cpu() for t in parts[1][:2])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(api.KcError):
+            ad.set(0, a, b)
+        ad.apply(x, rows, y, out=out)
+        with pytest.raises(api.KcError):
+            ad.clear(0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 def test_refusals(ctx):
     live = api.live_objects()
     for n_in, n_out, slots, rank in ((31, 8, 1, 4), (0, 8, 1, 4), (48, 8, 1, 4), (64, 0, 1, 4), (64, 8, 0, 4), (64, 8, 1, 0), (64, 8, 1, 129)):
