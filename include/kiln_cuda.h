@@ -444,8 +444,8 @@ KC_API int kc_paged_attention(kc_ctx_t ctx, kc_kv_t kv, int32_t layer, const voi
 
 /* The attention of a step as a handle, for callers that run it layer by layer, and for batches that share a long prefix: blocks
  * that sequences standing next to each other in `seqs` name at the same places of their tables, from the start on, are read
- * once for the rows of all of them, in pieces of 512 keys, where that saves enough (a model's own steps do the same); what
- * follows is each one's own. A row has the bits that kc_paged_attention gives it. The plan holds the step's description (seqs
+ * once for the rows of all of them, in pieces of 512 keys, where that saves enough and the memory for its partial results is
+ * there (a model's own steps do the same); what follows is each one's own. A row has the bits that kc_paged_attention gives it. The plan holds the step's description (seqs
  * and their tables are copied; sample_rows are not looked at) and a workspace; it belongs to the pools' context and is freed
  * before the pools. kc_attn_plan_set puts another step of the same heads and pools in its place, behind the runs queued before it,
  * and allocates only what the plan does not have yet: one plan serves a generation step after step. It is refused once a

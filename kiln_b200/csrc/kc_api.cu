@@ -193,6 +193,7 @@ struct kc_model {
   float* argmax_scratch = nullptr;     // per-CTA bests + counter of the fused reduction / arg-max of a streamed head
   float* partial_gu = nullptr;         // gate_up's fp32 partials while a gated down projection reads them (stream lane on)
   float* attn_ws = nullptr; size_t attn_ws_bytes = 0;
+  int attn_ws_refused = 0;             // steps to come that do not ask again for a workspace that they can do without
   // Query maps of ptr [rows tokens], boxes of `box` and ATT_SMALL_TOKENS tokens: of a step's own units, and of those over shared prefixes.
   struct QMaps { CUtensorMap map, small; const void* ptr = nullptr; int box = 0, rows = 0, gqa = 0; };
   QMaps q_maps[2];
@@ -1572,18 +1573,33 @@ int upload_meta(kc_model* m, kc_kv* kv, const uint32_t* token_ids, const kc_seq_
   return KC_OK;
 }
 
-int ensure_attn_ws(kc_model* m, const StepPlan& p) {
-  if (p.whole && !p.shared.on) return KC_OK;   // no partials
-  const size_t rows = (size_t)p.n * m->Hq * p.max_chunks;
+// Room for the partial results. A step whose own units need none takes those where there is no memory for what sharing needs, and so
+// do the steps behind it for a while: a wait for the stream and refused allocations in every one would cost more.
+int ensure_attn_ws(kc_model* m, StepPlan* p) {
+  constexpr int REFUSED_STEPS = 256;
+  if (p->whole && !p->shared.on) return KC_OK;   // no partials
+  const size_t rows = (size_t)p->n * m->Hq * p->max_chunks;
   const size_t need = rows * m->d.head_dim * 4 + rows * 8 + 256;
-  if (need > m->attn_ws_bytes) {
-    CK(cudaStreamSynchronize(m->ctx->stream));
-    cudaFree(m->attn_ws); m->attn_ws = nullptr; m->attn_ws_bytes = 0;
-    const size_t cap = align_up(need + need / 4, 1 << 20);
-    cudaError_t e = cudaMalloc(&m->attn_ws, cap);
-    if (e != cudaSuccess) return fail(KC_ERR_OOM, "attention workspace of %zu bytes: %s", cap, cudaGetErrorString(e));
-    m->attn_ws_bytes = cap;
+  if (need <= m->attn_ws_bytes) return KC_OK;
+  if (p->whole && m->attn_ws_refused > 0) {
+    --m->attn_ws_refused;
+    p->shared = StepPlan::Shared();
+    return KC_OK;
   }
+  CK(cudaStreamSynchronize(m->ctx->stream));
+  cudaFree(m->attn_ws); m->attn_ws = nullptr; m->attn_ws_bytes = 0;
+  size_t cap = align_up(need + need / 4, 1 << 20);
+  cudaError_t e = cudaMalloc(&m->attn_ws, cap);
+  if (e != cudaSuccess) { cudaGetLastError(); e = cudaMalloc(&m->attn_ws, cap = align_up(need, 256)); }
+  if (e == cudaSuccess) {
+    m->attn_ws_bytes = cap;
+    return KC_OK;
+  }
+  cudaGetLastError();
+  m->attn_ws = nullptr;
+  if (!p->whole) return fail(KC_ERR_OOM, "attention workspace of %zu bytes: %s", cap, cudaGetErrorString(e));
+  m->attn_ws_refused = REFUSED_STEPS;
+  p->shared = StepPlan::Shared();
   return KC_OK;
 }
 
@@ -1706,7 +1722,7 @@ bf16* tp_out_buffer(kc_model* m) {
 // The forward proper. tokens_dev: n u32 on the device (normally the metadata arena's copy).
 // greedy_out (optional, device; greedy_host: a pinned copy of it): where a single sampled row's raw arg-max goes when the head's reduction can produce
 // it itself (*greedy_done = true then; otherwise the caller samples from the logits as usual).
-int run_forward(kc_model* m, kc_kv* kv, const uint32_t* tokens_dev, const StepPlan& p, bool want_logits, uint32_t* greedy_out = nullptr,
+int run_forward(kc_model* m, kc_kv* kv, const uint32_t* tokens_dev, StepPlan& p, bool want_logits, uint32_t* greedy_out = nullptr,
                 bool* greedy_done = nullptr, uint32_t* greedy_host = nullptr) {
   kc_ctx* c = m->ctx;
   const kc_model_desc& d = m->d;
@@ -1715,7 +1731,7 @@ int run_forward(kc_model* m, kc_kv* kv, const uint32_t* tokens_dev, const StepPl
   const int32_t* token_pos = reinterpret_cast<const int32_t*>(m->meta_dev + p.lay.token_pos);
   const int32_t* kv_slot = reinterpret_cast<const int32_t*>(m->meta_dev + p.lay.kv_slot);
   int rc;
-  if ((rc = ensure_attn_ws(m, p))) return rc;
+  if ((rc = ensure_attn_ws(m, &p))) return rc;
   if ((rc = ensure_q_maps(m, m->q_rot, m->max_rows, m->Hq, m->Hq / m->Hkv, p))) return rc;
   const bool stream = m->stream_lane && n <= QL_STREAM_MAX_M && d.tp_world <= 1;
   // Per weight: the streaming kernel pays for itself from about 24 MB of records on (8B-class layers, every head); below
@@ -2146,7 +2162,7 @@ extern "C" int kc_paged_attention(kc_ctx_t c, kc_kv_t kv, int32_t layer, const v
   StepPlan p;
   rc = validate_step(m, kv, ids.data(), n, seqs, n_seqs, 0, &p, true, softcap > 0.f);
   if (!rc) rc = upload_meta(m, kv, ids.data(), seqs, p);
-  if (!rc) rc = ensure_attn_ws(m, p);
+  if (!rc) rc = ensure_attn_ws(m, &p);
   if (!rc) rc = ensure_q_maps(m, (const bf16*)q_dev, n, num_heads, num_heads / kv->kv_heads, p);
   // The kernels store 16 bytes at a time: an output that starts elsewhere gets a copy of an aligned one.
   const size_t out_bytes = (size_t)std::max(n, 1) * num_heads * kv->head_dim * sizeof(bf16);
@@ -2208,8 +2224,9 @@ static int set_attn_plan(kc_attn_plan* p, const kc_seq_step* seqs, int32_t n_seq
   p->plan[0].n = p->plan[1].n = 0;
   for (int i = 0; i < (apart ? 2 : 1); ++i) {
     RC(upload_meta(p->shell[i], p->kv, ids.data(), seqs, plan[i]));
-    RC(ensure_attn_ws(p->shell[i], plan[i]));
+    RC(ensure_attn_ws(p->shell[i], &plan[i]));
   }
+  if (!apart && !plan[0].shared.on) plan[1].shared = StepPlan::Shared();   // no memory for either
   p->apart = apart;
   for (int i = 0; i < 2; ++i) p->plan[i] = std::move(plan[i]);
   return KC_OK;

@@ -182,3 +182,84 @@ ok(rc); ok(rc_rows)
 for h in (r, who): lib.kc_adapter_rows_free(h)
 for h in (b, bank): lib.kc_adapters_free(h)
 """)
+
+
+SHARED = """
+ok(lib.kc_kv_create(ctx, 1, 8, 128, 400, 16, L.KC_BF16, C.byref(kv)))
+def behind(prefix, tails):
+    seqs, free = [], prefix // 16
+    for t in tails:
+        n = -(-(prefix + t + 1) // 16) - prefix // 16
+        ids = list(range(prefix // 16)) + list(range(free, free + n))
+        free += n
+        seqs.append((prefix + t, (C.c_uint32 * len(ids))(*ids)))
+    return (L.KcSeqStep * len(seqs))(*[L.KcSeqStep(1, off, 1, len(b), b) for off, b in seqs])
+tails = [3 + i for i in range(48)]
+seqs = behind(4096, tails)          # 48 x 32 heads x 9 chunks of 520 bytes: 7 MB
+"""
+
+
+def test_a_plan_without_memory_for_sharing(graphs):
+    """Sequences whose own units need no workspace are planned apart where the one for sharing is refused, with and without the margin."""
+    run(graphs, SHARED + """
+read, apart = C.c_int64(), C.c_int64()
+p = C.c_void_p()
+def shares():
+    ok(lib.kc_attn_plan_keys(p, C.byref(read), C.byref(apart)))
+    assert apart.value == sum(4096 + t + 1 for t in tails)
+    ok(lib.kc_attn_plan_run(p, 0, at, 0.1, 0.0, 0, at + (1 << 19)))
+    ok(lib.kc_attn_plan_run(p, 0, at, 0.1, 50.0, 0, at + (1 << 19)))
+    return read.value < apart.value
+fake.fake_fail_above(1 << 20)
+ok(lib.kc_attn_plan_create(ctx, kv, seqs, 48, 32, C.byref(p)))
+fake.fake_reset()
+assert not shares()
+assert calls() == ["launch in order"] * 2
+ok(lib.kc_attn_plan_set(p, seqs, 48))
+assert not shares() and "malloc" not in calls()   # not asked again at once
+fake.fake_fail_above(2 ** 62)
+for i in range(300):
+    ok(lib.kc_attn_plan_set(p, seqs, 48))
+assert shares() and calls().count("malloc") == 1
+lib.kc_attn_plan_free(p)
+fake.fake_fail_above(8 << 20)                     # room for what it needs
+ok(lib.kc_attn_plan_create(ctx, kv, seqs, 48, 32, C.byref(p)))
+assert shares()
+lib.kc_attn_plan_free(p)
+""")
+
+
+def test_a_step_without_memory_for_sharing(graphs):
+    """Forward, verify and decode steps run with the units that they would have without sharing."""
+    run(graphs, SHARED + """
+import dataclasses
+import numpy as np
+from kiln_b200 import api
+from kiln_b200.synth import PRESETS, synth_checkpoint
+fake.fake_shapes.restype = C.c_char_p
+cfg = dataclasses.replace(PRESETS["tiny-llama"], num_attention_heads=32, num_key_value_heads=8, head_dim=128, num_hidden_layers=1)
+c = api.Context(0)
+model = api.CudaModel(c, cfg, synth_checkpoint(cfg, seed=0), max_step_tokens=64, max_step_seqs=48)
+pool = api.PagedKv(c, model.kv_spec(400, 16))
+ids, feed, out = (C.c_uint32 * 48)(), (C.c_int32 * 48)(*[-1] * 48), (C.c_uint32 * 48)()
+logits, n, ticket, counts = C.c_void_p(), C.c_int32(), C.c_uint64(), (C.c_int32 * 48)()
+lib = L.lib()
+lib.kc_decode_launch.argtypes = L._SIGNATURES["kc_decode_launch"][1]
+def steps():
+    yield lib.kc_forward_step(model._h, pool._h, ids, 48, seqs, 48, 0, C.byref(logits), C.byref(n))
+    yield lib.kc_verify_step(model._h, pool._h, ids, 48, seqs, 48, out, counts, counts)
+    yield lib.kc_decode_launch(model._h, pool._h, ids, feed, seqs, 48, C.byref(ticket))
+def attention():
+    grids = []
+    for rc in steps():
+        assert rc == 0, lib.kc_last_error()
+        grids.append([s for s in fake.fake_shapes().decode().split() if s.split(":")[0] in ("384", "768")])
+        fake.fake_reset()
+    return grids
+fake.fake_fail_above(1 << 20)
+refused = attention()
+fake.fake_fail_above(2 ** 62)
+for _ in range(100): attention()
+shared = attention()
+assert refused[0] == refused[1] == refused[2] and shared[0] == shared[1] == shared[2] != refused[0], (refused, shared)
+""", first="import torch")
