@@ -1426,6 +1426,7 @@ void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& o
     });
   std::vector<AttnUnit> last;
   std::vector<AttnUnit>& others = resumes ? sh.rest : sh.units;
+  long long own_tiles = 0;   // of what the sequences take by themselves
   for (int i = 0; i < n; ++i)
     for (int t = 0; t < seqs[i].len; t += item) {
       AttnUnit u{};
@@ -1436,16 +1437,24 @@ void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& o
       for (int c = own(i); c < end; ++c) {
         u.chunk0 = c; u.chunk1 = c + 1;
         u.form = of_form(few, c == own(i) ? from[i] : 0);
+        own_tiles += (unit_keys(u) + 127) / 128;
         (c + 1 < end && unit_keys(u) == ATT_CHUNK ? others : last).push_back(u);
       }
     }
   std::stable_sort(last.begin(), last.end(), [](const AttnUnit& a, const AttnUnit& b) { return unit_keys(a) > unit_keys(b); });
   others.insert(others.end(), last.begin(), last.end());
-  // Tiles of 128 keys, the work of the SMs. Sharing costs 3 to 7 us more to begin with (partial results of every chunk and the kernel that
-  // merges them, units of more rows). Over 384 calls (four shapes of heads, 1 and 5 rows, 2 to 64 sequences, 512 to 8192 shared keys, tails of 40
-  // and 670), where it saves 3.5 tiles an SM it is up to 7.0 times as fast and at the worst 1.15 times as slow; where it saves
-  // fewer, it is left out at a loss of 2 % on average.
-  sh.on = (unit_tiles(p->units) - unit_tiles(sh.units) - unit_tiles(sh.rest)) * kv_heads * 2 >= 7ll * sm_count;
+  // Tiles of 128 keys, the work of the SMs: what sharing saves, in quarters. It costs 3 to 7 us more to begin with (partial results and the kernel
+  // that merges them, units of more rows), 3.5 tiles an SM; where the step's own units hold whole rows, half a tile for each unit more (its
+  // begin and end, its partial result); and where a wide run takes the kernel with a key per thread from sequences that would have it,
+  // a part of what those take by themselves. Over 1000 calls with both ways measured (five shapes of heads, 1 to 8 rows, 2 to 64 sequences that
+  // share 512 to 16384 keys, up to 126 others of 64 to 16384, tails of 20 to 4000; the weights are from 700 other ones) the better way of
+  // each call is on average 1.2 % faster than the rule's, and sharing at the worst 1.09 times as slow; by the 3.5 tiles alone 1.8 % and 1.49.
+  // 32 heads over 8 of 128 features, 5 rows, apart -> shared: 3 sequences behind 8192 beside 125 of 4096 379 -> 433 us, so they are
+  // left; 48 behind 4096 137 -> 60.
+  long long saved = 4 * (unit_tiles(p->units) - unit_tiles(sh.units) - unit_tiles(sh.rest));
+  if (p->whole) saved -= 2 * ((long long)sh.units.size() + (long long)sh.rest.size() - (long long)p->units.size());
+  if (p->keys && !sh.keys && !resumes) saved -= own_tiles * (head_dim > 128 ? 2 : p->whole ? 1 : 0);
+  sh.on = saved * kv_heads >= 14ll * sm_count;
   if (!sh.on) { sh.units.clear(); sh.rest.clear(); }
 }
 

@@ -263,3 +263,33 @@ for _ in range(100): attention()
 shared = attention()
 assert refused[0] == refused[1] == refused[2] and shared[0] == shared[1] == shared[2] != refused[0], (refused, shared)
 """, first="import torch")
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,k,prefix,others,length,capped,shared", [
+    (32, 8, 128, 5, 3, 8192, 125, 4096, False, False), (64, 8, 128, 5, 8, 4096, 100, 2048, False, False), (16, 8, 256, 1, 40, 1648, 81, 5088, True, False),
+    (32, 8, 128, 1, 3, 8192, 125, 4096, False, False), (28, 4, 128, 1, 8, 8192, 60, 4096, False, True), (32, 8, 128, 1, 16, 2048, 48, 2048, False, True),
+    (32, 8, 128, 5, 48, 4096, 0, 0, False, True), (32, 8, 128, 1, 48, 4096, 1, 60000, False, True), (64, 8, 128, 5, 64, 4096, 0, 0, False, True),
+    (32, 8, 64, 1, 64, 6001, 0, 0, False, True), (16, 8, 256, 4, 16, 6144, 0, 0, True, True)])
+def test_a_few_that_share_among_many(graphs, heads, kv_heads, hd, rows, k, prefix, others, length, capped, shared):
+    """Chunks read together make units of one chunk of every other sequence too: where few of a step share, what it costs the
+    others is weighed against it. Such steps were measured both ways, 7 % and more apart."""
+    run(graphs, f"""
+ok(lib.kc_kv_create(ctx, 1, {kv_heads}, {hd}, 6000, 16, L.KC_BF16, C.byref(kv)))
+full, tail, seqs, tables = {prefix} // 16, 40, [], []
+for i in range({k}):
+    n = -(-({prefix} + tail + {rows}) // 16) - full
+    tables.append((C.c_uint32 * (full + n))(*range(full), *(full + i * n + b for b in range(n))))
+    seqs.append(L.KcSeqStep({rows}, {prefix} + tail, 0, full + n, tables[-1]))
+for i in range({others}):                          # tables that agree nowhere
+    n = -(-({length} + {rows}) // 16)
+    tables.append((C.c_uint32 * n)(*((b + 7 * i) % 4000 + 2000 for b in range(n))))
+    seqs.append(L.KcSeqStep({rows}, {length}, 0, n, tables[-1]))
+p, read, apart = C.c_void_p(), C.c_int64(), C.c_int64()
+ok(lib.kc_attn_plan_create(ctx, kv, (L.KcSeqStep * len(seqs))(*seqs), len(seqs), {heads}, C.byref(p)))
+ok(lib.kc_attn_plan_keys(p, C.byref(read), C.byref(apart)))
+fake.fake_reset()
+ok(lib.kc_attn_plan_run(p, 0, at, 0.1, {50.0 if capped else 0.0}, 0, at + (1 << 19) * {1 if rows * (k + others) * heads * hd * 2 <= 1 << 19 else 100}))
+launched = len([c for c in calls() if c.startswith("launch")])
+if not {capped}: assert (read.value < apart.value) == {shared}, (read.value, apart.value)
+assert (launched > 1) == {shared}, launched
+""")
