@@ -448,7 +448,7 @@ class CudaModel:
         u = _uniforms(uniforms)
         if len(sampling) != p.n_seqs or u.shape != (n_sampled,):
             raise ValueError(f"{p.n_seqs} sequences and {n_sampled} sampled rows have {len(sampling)} settings and random numbers {u.shape}")
-        settings = (L.KcSampling * max(1, p.n_seqs))(*[L.KcSampling(s.temperature, s.top_k, s.top_p, s.min_p) for s in sampling])
+        settings = (L.KcSampling * max(1, p.n_seqs)).from_buffer_copy(_settings(sampling).tobytes().ljust(C.sizeof(L.KcSampling), b"\0"))
         rows, logprobs = np.zeros(max(1, n_sampled), dtype=np.uint32), np.zeros(max(1, n_sampled), dtype=np.float32)
         ncom, nacc = np.zeros(p.n_seqs, dtype=np.int32), np.zeros(p.n_seqs, dtype=np.int32)
         as_f32, as_i32 = C.POINTER(C.c_float), C.POINTER(C.c_int32)
@@ -564,10 +564,21 @@ class SamplingParams:
 _SAMPLING = np.dtype([("temperature", "f4"), ("top_k", "i4"), ("top_p", "f4"), ("min_p", "f4")])
 
 
+def _settings(params: Sequence[SamplingParams]) -> np.ndarray:
+    """The settings as kc_sampling records. A positive number stays one and a finite one too, whatever float32 has of it: a temperature
+    that rounds to 0 would be greedy, a top_p that does is refused by kc_verify_step_sampled."""
+    v = np.array([(p.temperature, p.top_p, p.min_p) for p in params], dtype=np.float64).reshape(-1, 3)
+    f = np.finfo(np.float32)
+    v = np.where(v > 0, np.clip(v, f.smallest_subnormal, f.max), v)
+    rec = np.empty(len(v), dtype=_SAMPLING)
+    rec["temperature"], rec["top_p"], rec["min_p"] = v.T
+    rec["top_k"] = [p.top_k for p in params]
+    return rec
+
+
 def pack_sampling(params: Sequence[SamplingParams], device) -> torch.Tensor:
     """The settings of a batch's rows as sample_rows takes them, int32 [rows, 4] on the device: made once, kept while they hold."""
-    rec = np.array([(p.temperature, p.top_k, p.top_p, p.min_p) for p in params], dtype=_SAMPLING)
-    return torch.from_numpy(rec.view(np.int32).reshape(-1, 4)).to(device)
+    return torch.from_numpy(_settings(params).view(np.int32).reshape(-1, 4)).to(device)
 
 
 def _uniforms(values) -> np.ndarray:

@@ -43,3 +43,12 @@ assert not [c for c in calls() if c.startswith("launch")]
 ok(sample()); ok(sample(logprobs=None)); ok(sample(rows=1, ld=0)); ok(sample(logits=at + 2, ld=101))
 assert len([c for c in calls() if c.startswith("launch")]) == 4
 """)
+
+
+def test_settings_that_float32_does_not_have():
+    """Positive and finite settings stay that: 0 and infinity have meanings of their own, and the verify round refuses a top_p of 0."""
+    tiny, large = float(np.finfo(np.float32).smallest_subnormal), float(np.finfo(np.float32).max)
+    got = api.pack_sampling([api.SamplingParams(1e-60, 0, 1e-46, 1e-300), api.SamplingParams(1e39), api.SamplingParams(0.0), api.SamplingParams(0.1, 3, 0.2, 0.3)], "cpu")
+    f = got.numpy().view(np.float32)
+    assert f[:, [0, 2, 3]].tolist() == [[tiny, tiny, tiny], [large, 1.0, 0.0], [0.0, 1.0, 0.0], [float(np.float32(x)) for x in (0.1, 0.2, 0.3)]]
+    assert got[:, 1].tolist() == [0, 0, 0, 3]
