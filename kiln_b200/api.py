@@ -569,7 +569,7 @@ def _settings(params: Sequence[SamplingParams]) -> np.ndarray:
     that rounds to 0 would be greedy, a top_p that does is refused by kc_verify_step_sampled."""
     v = np.array([(p.temperature, p.top_p, p.min_p) for p in params], dtype=np.float64).reshape(-1, 3)
     f = np.finfo(np.float32)
-    v = np.where(v > 0, np.clip(v, f.smallest_subnormal, f.max), v)
+    v = np.where((v > 0) & np.isfinite(v), np.clip(v, f.smallest_subnormal, f.max), v)
     rec = np.empty(len(v), dtype=_SAMPLING)
     rec["temperature"], rec["top_p"], rec["min_p"] = v.T
     rec["top_k"] = [p.top_k for p in params]
