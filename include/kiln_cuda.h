@@ -445,14 +445,17 @@ KC_API int kc_paged_attention(kc_ctx_t ctx, kc_kv_t kv, int32_t layer, const voi
 /* The attention of a step as a handle, for callers that run it layer by layer, and for batches that share a long prefix: blocks
  * that sequences standing next to each other in `seqs` name at the same places of their tables, from the start on, are read
  * once for the rows of all of them, in pieces of 512 keys, where that saves enough and the memory for its partial results is
- * there (a model's own steps do the same); what follows is each one's own. A row has the bits that kc_paged_attention gives it. The plan holds the step's description (seqs
- * and their tables are copied; sample_rows are not looked at) and a workspace; it belongs to the pools' context and is freed
- * before the pools. kc_attn_plan_set puts another step of the same heads and pools in its place, behind the runs queued before it,
- * and allocates only what the plan does not have yet: one plan serves a generation step after step. It is refused once a
- * graph has been captured over a run. kc_attn_plan_keys: keys that the plan reads for a kv head of a layer without a window,
- * and keys that it would read for every sequence apart. kc_attn_plan_run takes q bf16 [n, num_heads, head_dim] post-RoPE, n
- * the sum of the lens, and writes out bf16 [n, num_heads*head_dim], both 16-byte aligned and apart; scale, softcap and window
- * as in kc_paged_attention (a layer with a window reads every sequence's keys for itself). It expects the step's K/V in the
+ * there (a model's own steps do the same); what follows is each one's own. A step in which a sequence has more than 16
+ * tokens (a piece of a prompt) is read apart. A row has the bits that kc_paged_attention gives it.
+ * The plan holds the step's description (seqs and their tables are copied; sample_rows have no say) and a workspace: for a
+ * step that shares, n * num_heads * (4 * head_dim + 8) bytes for each 512 keys of its longest sequence. It belongs to the
+ * pools' context and is freed before the pools, and behind the last replay of a graph that holds a run of it.
+ * kc_attn_plan_set puts another step of the same heads and pools in its place, behind the runs queued before it, and
+ * allocates only what the plan does not have yet: one plan serves a generation step after step. It is refused once a graph
+ * has been captured over a run. kc_attn_plan_keys: keys that the plan reads for a kv head of a layer without a window, and
+ * keys that it would read for every sequence apart. kc_attn_plan_run takes q bf16 [n, num_heads, head_dim] post-RoPE, n the
+ * sum of the lens, and writes out bf16 [n, num_heads*head_dim], both 16-byte aligned and apart; scale, softcap and window as
+ * in kc_paged_attention (a layer with a window reads every sequence's keys for itself). It expects the step's K/V in the
  * pools by the time it runs, is asynchronous on the context's stream and may be captured. Runs of one plan share its
  * workspace: one after the other, graphs that hold them too. */
 typedef struct kc_attn_plan* kc_attn_plan_t;

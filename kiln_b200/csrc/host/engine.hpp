@@ -25,7 +25,8 @@
 // dispatch (VERIFY_MAX_KEY_LEN, deterministic width, per-model gamma) are inputs here.
 //
 // Out of scope (not on the verify path): preemption under pool exhaustion, priorities,
-// cancellation tokens, penalties, grammars, stochastic samplers. A step
+// cancellation tokens, penalties, grammars. Its requests are greedy: rows are drawn on the
+// device by kc_verify_step_sampled and kc_sample_rows, which a program calls itself. A step
 // that cannot get blocks for a plain decode slot returns a capacity error.
 #pragma once
 

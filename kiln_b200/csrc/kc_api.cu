@@ -1360,11 +1360,10 @@ long long unit_tiles(const std::vector<AttnUnit>& units) {
 // the chunk, as many as a unit holds, and every chunk's partial result is merged in index order as ever: a row has the bits
 // that it has alone. Of the chunk that a prefix ends in, the pieces of 128 keys that all have in common may be taken together
 // too; each sequence's unit then goes on from there, in a second launch.
-void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& old, int block_size, int head_dim, int gqa, int kv_heads, int sm_count,
-                 bool alone, bool capped) {
+void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& old, int block_size, int head_dim, int gqa, int kv_heads, int sm_count) {
   StepPlan::Shared& sh = p->shared;
   const int n = p->n_seqs, per = ATT_CHUNK / ATT_PIECE;
-  if (p->max_len > 16) return;   // a piece of a prompt: partial results of all its chunks would cost what is saved
+  if (p->max_len > 16) return;   // a step with a piece of a prompt keeps its own units: partial results of all the piece's chunks would cost what is saved
   // Pieces and chunks that a sequence shares with the one before it; first row; pieces that it does not take itself.
   std::vector<int> pieces(n + 1, 0), common(n + 1, 0), row(n + 1, 0), from(n, 0);
   int most = 0;
@@ -1498,7 +1497,7 @@ int validate_step(kc_model* m, kc_kv* kv, const uint32_t* token_ids, int32_t n, 
   p.max_chunks = (max_ctx + ATT_CHUNK - 1) / ATT_CHUNK;
   const std::vector<int> old = old_keys(kv, seqs, n_seqs);
   plan_attention(&p, seqs, old, m->d.head_dim, gqa, m->Hkv, m->ctx->sm_count, alone, capped);
-  if (share) plan_shared(&p, seqs, old, kv->block_size, m->d.head_dim, gqa, m->Hkv, m->ctx->sm_count, alone, capped);
+  if (share) plan_shared(&p, seqs, old, kv->block_size, m->d.head_dim, gqa, m->Hkv, m->ctx->sm_count);
   MetaLayout& L = p.lay;
   size_t at = 0;
   auto put = [&](size_t bytes) { size_t o = at; at = align_up(at + bytes, 16); return o; };

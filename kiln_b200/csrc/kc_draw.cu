@@ -12,15 +12,18 @@
 // summed in a fixed tree over the values, whatever the number of CTAs a row has.
 //
 // Counting: a bin a value, of the magnitudes [2^-25, 2^7) of either sign (the home window), 32 KB of shared memory. A row with
-// other magnitudes (but for -inf, and one smaller value of either sign, as a row in five hundred has) takes another pass over itself for each
-// of the eight other windows of 32 binary orders that it has values in, so that any row is exact; zeros are counted apart. The counts and masses of the binades lie in shared memory of every CTA of the row's
-// cluster, which then all look for the same borders. A bin also adds up where its values stand, so that a value that a CTA has once
-// is found without another pass: 512 rows of 256000 took 159 -> 141 us.
+// other magnitudes (but for -inf, and one smaller value of either sign, as a row in five hundred has) takes another pass over
+// itself for each of the eight other windows of 32 binary orders that it has values in, so that any row is exact; zeros are
+// counted apart. The counts and masses of the binades lie in shared memory of every CTA of the row's cluster, which then all look
+// for the same borders. A bin also adds up where its values stand, so that a value that a CTA has once is found without
+// another pass: 512 rows of 256000 took 159 -> 141 us.
 //
-// What bounds it. Few rows: launch, three cluster barriers and the search's chains of latencies, 2200 cycles a border: one row of 128256 11.6 us,
-// seven of 50001 13.1. Many: the counting, at 0.7 of what shared memory's atomics take (3.6 wavefronts for a warp's 32 places), and
-// behind it the accounts and the search, 17000 cycles that only the SM's other CTAs can fill: 128 rows of 128256 24.5 us, 192 31.9 (384 CTAs
-// in 444 places; 7.5 us at a copy's rate), 512 of 256000 102 (40). One CTA a row 47 at 192.
+// What bounds it. Few rows: launch, three cluster barriers and the search's chains of latencies, 2200 cycles a border: one row of
+// 128256 11.6 us, seven of 50001 13.1. Many: the counting, at 0.7 of what shared memory's atomics take (3.6 wavefronts for a warp's 32
+// places), and behind it the accounts and the search, 17000 cycles that only the SM's other CTAs can fill: 128 rows of 128256
+// 24.5 us, 192 31.9 (384 CTAs in 444 places; 7.5 us at a copy's rate), 512 of 256000 102 (40). One CTA a row 47 at 192. Masked tokens
+// all meet in one bin, whose atomics come one after the other, and a finite mask's window takes passes of its own: 192 rows of
+// 128256 with 99 % of -inf take 115 us, of the type's lowest value 240 (30 without).
 #include "kc_fused.cuh"
 #include "kc_umma.cuh"
 

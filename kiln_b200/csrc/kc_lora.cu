@@ -14,10 +14,11 @@
 // of the product (2048 rows of rank 64: 118 -> 94 us without). y is added in fp32 and the result rounded once.
 //
 // What bounds it. Few rows: launch, two latencies of memory and two exchanges, 4.8 us; 32 rows of an adapter each into 28672 features
-// read 29 MB of B in 13.4 us, of which 5.7 are memory's. Many rows: the 16 rows of a tile share what they read of B, so that
-// L1 sees four times y; 2048 rows of rank 64 into 28672 features take 89 us, 44 at a copy's rate. Tiles of 32 and 64 rows with B through
-// shared memory were built and are no faster (94 and 155 us at these sizes): a CTA's fixed part, a barrier a round and fewer clusters at once
-// cost what they save.
+// read 29 MB of B in 12.5 us, of which 5.7 are memory's. Many rows: the 16 rows of a tile share what they read of B, so that
+// L1 sees four times y; 2048 rows of rank 64 into 28672 features take 88 us, 44 at a copy's rate. Tiles of 32 and 64 rows with B and y
+// through a ring of shared memory took 74 and 110 us there, but the smaller of them 61 for 46 from 14336 to 4096 features, 58 for 49 at
+// 1024 rows and 37 for 24 at 256: how many clusters the SMs hold at once weighs more than what is read of B. Every slot costs
+// the ranks of the bank's stride: rank 8 or 16 into 28672 features for 32 adapters 9.4 us from L2, 27 in a bank of rank 64.
 #include "kc_lora.cuh"
 
 #include "kc_umma.cuh"
@@ -273,7 +274,7 @@ cudaError_t launch(const LoraParams& p, cudaStream_t s) {
 
 // The largest clusters of which the SMs hold all at once (a cluster lies in one group of SMs: of 296 places for CTAs clusters of eight
 // take 256, of seven and six 252, of four 284, of three 270), else two CTAs a tile, whose fixed part weighs least. 4096 -> 28672 features,
-// rank 16, us with 8, 7, 6, 4, 3 and 2 CTAs: 32 tiles 11.7, 13.1, 13.9, -, -, -; 34 17.6, 14.0, 14.7; 38 20.3, 21.7, 15.2, 18.3; 46 -, 26.8, 27.1, 21.3; 72
+// rank 16, the kernel's us by itself with 8, 7, 6, 4, 3 and 2 CTAs: 32 tiles 11.7, 13.1, 13.9, -, -, -; 34 17.6, 14.0, 14.7; 38 20.3, 21.7, 15.2, 18.3; 46 -, 26.8, 27.1, 21.3; 72
 // -, -, -, 44.6, 34.7, 41; 94 -, -, -, -, 57.6, 44.9. Clusters of five gain 8 % on four at 46 to 53 tiles.
 template <int R>
 cudaError_t launch_rank(const LoraParams& p, int sm_count, cudaStream_t s) {
