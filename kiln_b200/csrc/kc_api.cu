@@ -2214,9 +2214,11 @@ static bool same_units(const std::vector<AttnUnit>& a, const std::vector<AttnUni
 // Plans `seqs` into the handle. Buffers grow where they have to, so that a plan set step after step allocates nothing; the host waits
 // for the copies of two settings before at the most. Refused sequences leave the plan as it was; a failed copy or allocation
 // leaves it without one.
-static int set_attn_plan(kc_attn_plan* p, const kc_seq_step* seqs, int32_t n_seqs, const char* where) {
+static int set_attn_plan(kc_attn_plan* p, const kc_seq_step* step, int32_t n_seqs, const char* where) {
+  std::vector<kc_seq_step> copy(step, step + std::max(0, n_seqs));   // nothing is sampled, whatever they say
+  const kc_seq_step* seqs = copy.data();
   long long n = 0;
-  for (int i = 0; i < n_seqs; ++i) n += std::max(0, seqs[i].len);
+  for (kc_seq_step& s : copy) { n += std::max(0, s.len); s.sample_rows = 0; }
   if (n_seqs < 1 || n < 1 || n > 1 << 24) return fail(KC_ERR_INVALID, "%s: %lld token(s) of %d sequence(s)", where, n, n_seqs);
   RC(not_captured(p->ctx, where));
   std::vector<uint32_t> ids((size_t)n, 0);

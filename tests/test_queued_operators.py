@@ -293,3 +293,17 @@ launched = len([c for c in calls() if c.startswith("launch")])
 if not {capped}: assert (read.value < apart.value) == {shared}, (read.value, apart.value)
 assert (launched > 1) == {shared}, launched
 """)
+
+
+@pytest.mark.parametrize("sample_rows", [-1, 0, 3, 4, 2 ** 31 - 1])
+def test_a_plan_samples_nothing(graphs, sample_rows):
+    """sample_rows have no say in a plan: neither in whether it is taken nor in what it holds."""
+    run(graphs, f"""
+p = C.c_void_p()
+seqs = (L.KcSeqStep * 2)(L.KcSeqStep(3, 40, {sample_rows}, 3, table), L.KcSeqStep(1, 7, {sample_rows}, 1, table))
+ok(lib.kc_attn_plan_create(ctx, kv, seqs, 2, 4, C.byref(p)))
+ok(lib.kc_attn_plan_set(p, seqs, 2))
+assert seqs[0].sample_rows == seqs[1].sample_rows == {sample_rows}
+ok(lib.kc_attn_plan_run(p, 0, at, 0.1, 0.0, 0, at + 4096))
+lib.kc_attn_plan_free(p)
+""")
