@@ -1393,9 +1393,11 @@ void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& o
   const int item = p->tokens_per_item;
   // The second launch, and its units' way into what they go on from, cost 6 to 10 us. Over 386 calls (five shapes of heads, 1 and 4 rows, 8 to
   // 128 sequences, tails of 40 and 300) it is 0.83 of the time without where it saves 10 to 20 tiles an SM, 0.68 beyond, 0.98 at
-  // 6 to 10, 1.04 at 4 to 6, 1.3 at 1.
+  // 6 to 10, 1.04 at 4 to 6, 1.3 at 1. It is of the kernel with a key per thread: where the step's own units take the other one, chunks
+  // of their own by that are 0.88 of the time on average of 49 calls (108 sequences behind 2432, 64 heads over 8 of 64 features, 8 rows:
+  // 1.08 of the step apart -> 0.89), and slower in two.
   bool resumes = false;
-  if (item * gqa <= KEY_ROWS) {
+  if (p->keys && item * gqa <= KEY_ROWS) {
     const int per_unit = std::max(1, ATT_ROWS / gqa);
     long long saved = 0;
     partly_runs([&](int i, int r0, int r1, int j, int k) { saved += (long long)k * (j - i + 1 - (r1 - r0 + per_unit - 1) / per_unit); });

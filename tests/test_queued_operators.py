@@ -307,3 +307,23 @@ assert seqs[0].sample_rows == seqs[1].sample_rows == {sample_rows}
 ok(lib.kc_attn_plan_run(p, 0, at, 0.1, 0.0, 0, at + 4096))
 lib.kc_attn_plan_free(p)
 """)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,k,prefix,launches", [
+    (64, 8, 64, 8, 108, 2432, 2), (64, 8, 128, 8, 173, 2448, 2), (32, 8, 64, 1, 128, 6001, 3), (32, 8, 128, 4, 250, 2448, 3)])
+def test_a_chunk_in_part_is_gone_on_from_where_the_kernel_is_the_faster_one(graphs, heads, kv_heads, hd, rows, k, prefix, launches):
+    """The launch that goes on from the shared pieces of a chunk is of the kernel with a key per thread; where a step's own
+    units take the other one, a chunk that is shared in part is each sequence's own."""
+    run(graphs, f"""
+ok(lib.kc_kv_create(ctx, 1, {kv_heads}, {hd}, 6000, 16, L.KC_BF16, C.byref(kv)))
+full, seqs, tables = {prefix} // 16, [], []
+for i in range({k}):
+    n = -(-({prefix} + 40 + {rows}) // 16) - full
+    tables.append((C.c_uint32 * (full + n))(*range(full), *(full + i * n + b for b in range(n))))
+    seqs.append(L.KcSeqStep({rows}, {prefix} + 40, 0, full + n, tables[-1]))
+p = C.c_void_p()
+ok(lib.kc_attn_plan_create(ctx, kv, (L.KcSeqStep * len(seqs))(*seqs), len(seqs), {heads}, C.byref(p)))
+fake.fake_reset()
+ok(lib.kc_attn_plan_run(p, 0, at, 0.1, 0.0, 0, at + (1 << 28)))
+assert len([c for c in calls() if c.startswith("launch")]) == {launches}
+""")
