@@ -1444,16 +1444,21 @@ void plan_shared(StepPlan* p, const kc_seq_step* seqs, const std::vector<int>& o
     }
   std::stable_sort(last.begin(), last.end(), [](const AttnUnit& a, const AttnUnit& b) { return unit_keys(a) > unit_keys(b); });
   others.insert(others.end(), last.begin(), last.end());
-  // Tiles of 128 keys, the work of the SMs: what sharing saves, in quarters. It costs 3 to 7 us more to begin with (partial results and the kernel
-  // that merges them, units of more rows), 3.5 tiles an SM; where the step's own units hold whole rows, half a tile for each unit more (its
-  // begin and end, its partial result); and where a wide run takes the kernel with a key per thread from sequences that would have it,
-  // a part of what those take by themselves. Over 1000 calls with both ways measured (five shapes of heads, 1 to 8 rows, 2 to 64 sequences that
-  // share 512 to 16384 keys, up to 126 others of 64 to 16384, tails of 20 to 4000; the weights are from 700 other ones) the better way of
-  // each call is on average 1.2 % faster than the rule's, and sharing at the worst 1.09 times as slow; by the 3.5 tiles alone 1.8 % and 1.49.
-  // 32 heads over 8 of 128 features, 5 rows, apart -> shared: 3 sequences behind 8192 beside 125 of 4096 379 -> 433 us, so they are
-  // left; 48 behind 4096 137 -> 60.
+  // Tiles of 128 keys, the work of the SMs: what sharing saves, in quarters. It costs 3 to 7 us more to begin with (units of more rows, the
+  // kernel that merges), 3.5 tiles an SM; where the step's own units hold whole rows, half a tile for each unit more (its begin and end)
+  // and the partial results of all rows, written and read, 64 of a row and head being the bytes of a tile; and where a wide run takes the
+  // kernel with a key per thread from sequences that would have it, a part of what those take by themselves. Over 2000 calls with both
+  // ways measured (14 shapes of heads, 1 to 16 rows, 2 to 250 sequences that share 512 to 16384 keys, up to 200 others of 64 to 16384, tails of
+  // 20 to 4000; the weights are from 1700 other ones) the better way of each call is on average 1.0 % faster than the rule's, and sharing
+  // at the worst 1.26 times as slow; by the 3.5 tiles alone 2.6 % and 1.58. 32 heads over 8 of 128 features, 5 rows, apart -> shared: 3
+  // sequences behind 8192 beside 125 of 4096 379 -> 433 us, so they are left; 48 behind 4096 137 -> 60.
   long long saved = 4 * (unit_tiles(p->units) - unit_tiles(sh.units) - unit_tiles(sh.rest));
-  if (p->whole) saved -= 2 * ((long long)sh.units.size() + (long long)sh.rest.size() - (long long)p->units.size());
+  if (p->whole) {
+    long long partials = 0;   // of a head
+    for (int i = 0; i < n; ++i)
+      for (int t = 0; t < seqs[i].len; ++t) partials += (seqs[i].offset + t) / ATT_CHUNK + 1;
+    saved -= 2 * ((long long)sh.units.size() + (long long)sh.rest.size() - (long long)p->units.size()) + partials * gqa / 16;
+  }
   if (p->keys && !sh.keys && !resumes) saved -= own_tiles * (head_dim > 128 ? 2 : p->whole ? 1 : 0);
   sh.on = saved * kv_heads >= 14ll * sm_count;
   if (!sh.on) { sh.units.clear(); sh.rest.clear(); }

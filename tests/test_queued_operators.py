@@ -327,3 +327,27 @@ fake.fake_reset()
 ok(lib.kc_attn_plan_run(p, 0, at, 0.1, 0.0, 0, at + (1 << 28)))
 assert len([c for c in calls() if c.startswith("launch")]) == {launches}
 """)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,k,prefix,others,length,shared", [
+    (28, 4, 128, 8, 211, 896, 49, 74, False), (64, 8, 128, 8, 89, 1424, 180, 706, False), (64, 8, 128, 8, 219, 896, 0, 0, False),
+    (64, 8, 128, 8, 173, 2448, 0, 0, True), (64, 8, 64, 8, 108, 2432, 0, 0, True)])
+def test_partial_results_of_many_rows(graphs, heads, kv_heads, hd, rows, k, prefix, others, length, shared):
+    """Rows of wide groups: what they leave for a chunk and what is merged is as much as the chunk's keys. Measured both ways, 8 % and
+    more apart."""
+    run(graphs, f"""
+ok(lib.kc_kv_create(ctx, 1, {kv_heads}, {hd}, 6000, 16, L.KC_BF16, C.byref(kv)))
+full, seqs, tables = {prefix} // 16, [], []
+for i in range({k}):
+    n = -(-({prefix} + 40 + {rows}) // 16) - full
+    tables.append((C.c_uint32 * (full + n))(*range(full), *(full + i * n + b for b in range(n))))
+    seqs.append(L.KcSeqStep({rows}, {prefix} + 40, 0, full + n, tables[-1]))
+for i in range({others}):                          # tables that agree nowhere
+    n = -(-({length} + {rows}) // 16)
+    tables.append((C.c_uint32 * n)(*((b + 7 * i) % 2000 + 4000 for b in range(n))))
+    seqs.append(L.KcSeqStep({rows}, {length}, 0, n, tables[-1]))
+p, read, apart = C.c_void_p(), C.c_int64(), C.c_int64()
+ok(lib.kc_attn_plan_create(ctx, kv, (L.KcSeqStep * len(seqs))(*seqs), len(seqs), {heads}, C.byref(p)))
+ok(lib.kc_attn_plan_keys(p, C.byref(read), C.byref(apart)))
+assert (read.value < apart.value) == {shared}, (read.value, apart.value)
+""")
